@@ -121,6 +121,10 @@ def fp8_linear(x_fp8: torch.Tensor, x_scale: torch.Tensor, w_fp8: torch.Tensor, 
     return _native.fp8_linear(x_fp8, x_scale, w_fp8, w_scale, out, packed, k_split)
 
 
+from .paged import (PagedKVCache, PagedPlan, RopeFrequencies, paged_attention, paged_keep, paged_plan, rope, rope_frequencies,  # noqa: E402,F401
+                    rope_paged)
+
+
 class _TorchOps:
     """The operator set GPUKDistEnv drives; tests substitute a recording fake."""
     init_ar_fusion = staticmethod(init_ar_fusion)

@@ -27,7 +27,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
 ]
 CORE_SOURCES = ["core.cu", "launch_bf16.cu", "launch_f16.cu", "launch_f32.cu", "noalloc.cu", "fp8_linear.cu", "stream_linear.cu", "tensor_map.cu", "decoder_ops.cu",
-                "attention.cu", "prefill_attention.cu"]
+                "attention.cu", "prefill_attention.cu", "paged_ops.cu", "paged_attention.cu", "rope.cu"]
 HEADERS = ["common.cuh", "epilogue.cuh", "kernels.cuh", "launch.cuh", "launch_impl.cuh", "linear.cuh", "tensor_core.cuh", "decoder_math.cuh",
            os.path.join(ROOT, "include", "gpuk_b200.h")]
 
@@ -71,8 +71,8 @@ def build_torch(verbose: bool = False, force: bool = False) -> str:
     import torch
     from torch.utils import cpp_extension as ce
 
-    srcs = [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "native.cpp")]
-    deps = srcs + [os.path.join(ROOT, "include", "gpuk_b200.h"), CORE_LIB]
+    srcs = [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "native.cpp"), os.path.join(CSRC, "native_paged.cpp")]
+    deps = srcs + [os.path.join(CSRC, "native.hpp"), os.path.join(ROOT, "include", "gpuk_b200.h"), CORE_LIB]
     if not force and _newer(TORCH_LIB, deps):
         return TORCH_LIB
     import sysconfig

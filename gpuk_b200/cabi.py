@@ -29,6 +29,12 @@ class Plan(ctypes.Structure):
                 ("ws", c_int), ("ws_grid", c_int), ("ws_vpt", c_int), ("ws_tf", c_int), ("ws_tr", c_int), ("ws_ts", c_int)]
 
 
+class Pages(ctypes.Structure):
+    """gpuk_pages: one layer's keys and values, strides in values."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64), ("row_stride", c_int64), ("num_pages", c_int64),
+                ("kv_heads", c_int), ("page_size", c_int), ("head_dim", c_int), ("dtype", c_int)]
+
+
 class GpukError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"gpuk status {status}: {message}")
@@ -87,6 +93,13 @@ _SIGNATURES = {
     "gpuk_prefill_attention": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "gpuk_rope_append": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "gpuk_silu_mul": (c_int, [_P, _P, c_int64, c_int, _P]),
+    "gpuk_paged_plan": (c_int, [_P, _P, _P, c_int64, c_int, _P, _P, c_int, _P, _P] + [c_int] * 4 + [_P] * 7),
+    "gpuk_rope": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, c_float] + [c_int] * 6 + [_P]),
+    "gpuk_rope_paged": (c_int, [_P, c_int64, c_int64] * 4 + [_P, _P, _P, c_float, POINTER(Pages)] + [c_int] * 4 + [_P]),
+    "gpuk_paged_attention_workspace": (c_int, [POINTER(Pages), c_int, c_int, c_int, c_int64, POINTER(c_int64)]),
+    "gpuk_paged_attention": (c_int, [_P, c_int64, c_int64, POINTER(Pages), _P, c_int64, c_int, _P, _P, _P, c_int, _P, c_int64, c_int64, c_int, c_int, c_int, c_int64,
+                                     c_float, _P, c_int64, _P]),
+    "gpuk_paged_keep": (c_int, [POINTER(Pages), c_int, c_int64, _P, c_int64, c_int, _P, _P, c_int64, c_int, _P, c_int, _P]),
 }
 for _name, (_res, _args) in _SIGNATURES.items():
     _fn = getattr(lib, _name)

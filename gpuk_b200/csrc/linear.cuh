@@ -40,6 +40,8 @@ struct DecodeDevice {
 cudaError_t stream_linear_setup(DecodeDevice *d);          // once per device
 cudaError_t decode_attention_setup(DecodeDevice *d);
 cudaError_t prefill_attention_setup();
+cudaError_t paged_attention_setup();
+cudaError_t paged_ops_setup();
 constexpr int kStatusPosition = 1, kDecodeStatusWords = 2;
 // The current device; the first call on it opts the kernels in to their shared memory, so that no later call has set-up left to do.
 int decode_device(const DecodeDevice **device);

@@ -4,70 +4,12 @@
 // neither of those: a call through them costs several microseconds of host time, which is what bounds a step of a few sequences
 // (fused epilogue, 8 rows: 11.0 -> 6.6 us a call; FP8 linear layer, 8 tokens, 1280 x 8192: 14.8 -> 5.7 us).  All but fp8_linear return None for a
 // call that belongs to the operators: see NotDirect and add_rms.
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
+#include "native.hpp"
 
-#include <climits>
-
-#include "gpuk_b200.h"
-
-using at::Tensor;
+using namespace gpuk_native;
 
 namespace {
 
-void check(int status, const char *what) {
-    TORCH_CHECK(status == GPUK_OK, "gpuk::", what, ": ", gpuk_status_string(status), ": ", gpuk_last_error());
-}
-
-const Tensor &tensor_arg(PyObject *o, const char *what) {
-    TORCH_CHECK(THPVariable_Check(o), "gpuk: ", what, " must be a tensor");
-    return THPVariable_Unpack(o);
-}
-int64_t int_arg(PyObject *o) {
-    const int64_t v = PyLong_AsLongLong(o);
-    if (v == -1 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-// A size as the C ABI takes it.
-int int_size(int64_t v) {
-    TORCH_CHECK(v >= 0 && v <= INT_MAX, "gpuk: a size of ", v, " is out of range");
-    return static_cast<int>(v);
-}
-struct NoGil {
-    PyThreadState *state = PyEval_SaveThread();
-    ~NoGil() { PyEval_RestoreThread(state); }
-};
-void expect_args(Py_ssize_t n, Py_ssize_t want, const char *what) { TORCH_CHECK(n == want, "gpuk::", what, " takes ", want, " arguments, got ", n); }
-void *stream_of(const Tensor &t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
-Tensor empty_like_on(const Tensor &t, at::IntArrayRef sizes, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt); }
-
-// A tensor whose operators would go straight to the CUDA kernels: of the class Tensor itself, dense and contiguous, no transform or lazy bit on it.
-bool plain_class(PyObject *o) {
-    if (!THPVariable_CheckExact(o)) return false;
-    const Tensor &t = THPVariable_Unpack(o);
-    static const c10::DispatchKeySet other({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
-                                            c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Batched, c10::DispatchKey::Negative, c10::DispatchKey::Conjugate,
-                                            c10::DispatchKey::ZeroTensor, c10::DispatchKey::NestedTensor});
-    return !t.key_set().has_any(other);
-}
-bool plain(PyObject *o, int device) {
-    if (!plain_class(o)) return false;
-    const Tensor &t = THPVariable_Unpack(o);
-    return t.is_cuda() && (device < 0 || t.get_device() == device) && t.layout() == at::kStrided && t.is_contiguous();
-}
-// No mode that wants to see operators: tracing, functional transforms, dispatch or function modes.
-bool no_modes() {
-    const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
-    static const c10::DispatchKeySet front({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Functionalize,
-                                            c10::DispatchKey::Tracer, c10::DispatchKey::Python, c10::DispatchKey::PreDispatch});
-    return !tls.included_.has_any(front) && !c10::impl::TorchDispatchModeTLS::any_modes_set() && at::impl::PythonTorchFunctionTLS::stack_len() == 0;
-}
 // Thrown for a tensor that a decode call below does not read as it is: it returns None, and the caller takes the operators, which accept any strides and types that go
 // together.
 struct NotDirect {};
@@ -360,9 +302,6 @@ PyObject *no_modes_py(PyObject *, PyObject *) {
     END_HANDLE_TH_ERRORS
 }
 
-template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
-constexpr PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)); }
-
 PyMethodDef methods[] = {
     {"no_modes", no_modes_py, METH_NOARGS, nullptr},
     {"rope_append", fast<rope_append>(), METH_FASTCALL, nullptr},
@@ -374,6 +313,11 @@ PyMethodDef methods[] = {
     {"fp8_linear", fast<fp8_linear>(), METH_FASTCALL, nullptr},
     {"add_rms", fast<add_rms>(), METH_FASTCALL, nullptr},
     {"silu_mul", fast<silu_mul>(), METH_FASTCALL, nullptr},
+    {"paged_plan", fast<paged_plan>(), METH_FASTCALL, nullptr},
+    {"rope", fast<rope>(), METH_FASTCALL, nullptr},
+    {"rope_paged", fast<rope_paged>(), METH_FASTCALL, nullptr},
+    {"paged_attention", fast<paged_attention>(), METH_FASTCALL, nullptr},
+    {"paged_keep", fast<paged_keep>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "gpuk_b200._native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,320 @@
+// What keeps a paged KV cache between the passes of attention over it, one launch each:
+//
+//   plan_kernel   block tables made to fit the requests' lengths, and for each new token its position, its slot and, in a tree of drafts, its ancestors.
+//   keep_kernel   the keys and values of a tree's accepted path moved to the end of the cached tokens, in all layers.
+//
+// Both move little and are bound by latency: a plan is one cluster that reads the lengths once and meets once, in place of the dozen operators (prefix sums, searches,
+// scatters) that it takes otherwise; the moves of a path read eight rows ahead of their writes.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/gpuk_b200.h"
+#include "common.cuh"
+#include "launch.cuh"
+#include "linear.cuh"
+
+namespace gpuk {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kMaxRequests = 4096;
+constexpr int kMaxWords = 8;
+
+struct PlanParams {
+    const int32_t *lens, *new_lens, *held, *free_count, *parents;
+    int32_t *tables, *free;
+    int32_t *starts, *masks, *held_out, *free_count_out;
+    int64_t *positions, *slots;
+    int64_t table_stride;
+    int batch, width, page_shift, capacity, total, words;
+};
+
+// Sums of a, b and c over the threads in front, and over all of them.
+struct Sums {
+    int64_t a, b, c;
+};
+__device__ Sums block_before(Sums v, Sums *all, Sums (&warp_sums)[kPlanWarps]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Sums s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const Sums t = {__shfl_up_sync(0xffffffffu, s.a, o), __shfl_up_sync(0xffffffffu, s.b, o), __shfl_up_sync(0xffffffffu, s.c, o)};
+        if (lane >= o) s.a += t.a, s.b += t.b, s.c += t.c;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = s;
+    __syncthreads();
+    Sums w = warp_sums[lane], u = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const Sums t = {__shfl_up_sync(0xffffffffu, u.a, o), __shfl_up_sync(0xffffffffu, u.b, o), __shfl_up_sync(0xffffffffu, u.c, o)};
+        if (lane >= o) u.a += t.a, u.b += t.b, u.c += t.c;
+    }
+    *all = {__shfl_sync(0xffffffffu, u.a, 31), __shfl_sync(0xffffffffu, u.b, 31), __shfl_sync(0xffffffffu, u.c, 31)};
+    const Sums f = {__shfl_sync(0xffffffffu, u.a - w.a, warp), __shfl_sync(0xffffffffu, u.b - w.b, warp), __shfl_sync(0xffffffffu, u.c - w.c, warp)};
+    return {f.a + s.a - v.a, f.b + s.b - v.b, f.c + s.c - v.c};
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams p) {
+    extern __shared__ int32_t lists[];      // per request: first token, the pages in front that come back or go out, and those that it holds
+    __shared__ Sums warp_sums[kPlanWarps];
+    int32_t *const starts = lists, *const back_at = starts + p.batch + 1, *const want_at = back_at + p.batch, *const holds = want_at + p.batch;
+    const int ctas = cluster_size(), cta = cluster_cta_rank(), tid = threadIdx.x, lane = tid & 31;
+    const int64_t thread = static_cast<int64_t>(cta) * kPlanThreads + tid, threads = static_cast<int64_t>(ctas) * kPlanThreads;
+    grid_dependency_sync();
+    const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
+    const int page = 1 << p.page_shift;
+
+    struct Need {
+        int64_t lens;
+        int held, need;
+        int64_t over;
+    };
+    auto need_of = [&](int i, int n) {
+        Need r;
+        r.lens = max(p.lens[i], 0);
+        const int64_t pages = (r.lens + n + page - 1) >> p.page_shift;
+        r.held = holds[i];
+        r.need = static_cast<int>(min(pages, static_cast<int64_t>(p.width)));
+        r.over = pages - r.need;
+        return r;
+    };
+    // every CTA goes over all requests: starts, and how many pages come back and go out in front of each
+    int64_t tokens = 0;
+    Sums pages = {0, 0, 0};
+    for (int base = 0; base < p.batch; base += kPlanThreads) {
+        const int i = base + tid;
+        const bool here = i < p.batch;
+        Sums all;
+        const int64_t n_given = here ? max(p.new_lens[i], 0) : 0;
+        const int64_t first = min(tokens + block_before({n_given, 0, 0}, &all, warp_sums).a, static_cast<int64_t>(p.total));
+        const int n = static_cast<int>(min(n_given, p.total - first));
+        tokens += all.a;
+        Sums v = {0, 0, 0};
+        if (here) {
+            holds[i] = min(max(p.held[i], 0), p.width);
+            const Need r = need_of(i, n);
+            v = {max(r.held - r.need, 0), max(r.need - r.held, 0), r.over};
+        }
+        const Sums before = block_before(v, &all, warp_sums);
+        if (here) {
+            starts[i] = static_cast<int32_t>(first);
+            back_at[i] = static_cast<int32_t>(pages.a + before.a), want_at[i] = static_cast<int32_t>(pages.b + before.b);
+        }
+        pages.a += all.a, pages.b += all.b, pages.c += all.c;
+    }
+    if (tid == 0) starts[p.batch] = static_cast<int32_t>(min(tokens, static_cast<int64_t>(p.total)));
+    const int count = min(max(p.free_count[0], 0), p.capacity);
+    const int there = static_cast<int>(min(count + pages.a, static_cast<int64_t>(p.capacity)));
+    __syncthreads();
+    // pages that are too many, onto the list: a warp per request
+    for (int i = static_cast<int>(thread / 32); i < p.batch; i += static_cast<int>(threads / 32)) {
+        const Need r = need_of(i, starts[i + 1] - starts[i]);
+        for (int j = r.need + lane; j < r.held; j += 32) {
+            const int64_t at = static_cast<int64_t>(count) + back_at[i] + j - r.need;
+            if (at < p.capacity) p.free[at] = p.tables[i * p.table_stride + j];
+        }
+    }
+    cluster_barrier();      // the list is whole, and everybody has read the counts: they may be written where they came from
+    auto page_from = [&](int i, int nth) {
+        const int64_t at = static_cast<int64_t>(there) - 1 - (static_cast<int64_t>(want_at[i]) + nth);
+        return at >= 0 ? p.free[at] : -1;
+    };
+    // positions, slots and ancestors
+    const int seen = starts[p.batch];
+    for (int64_t t = thread; t < p.total; t += threads) {
+        int64_t position = -1, slot = -1;
+        uint32_t bits[kMaxWords] = {};
+        if (t < seen) {
+            int lo = 0, hi = p.batch;      // starts[lo] <= t < starts[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (starts[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            const int first = starts[lo], index = static_cast<int>(t) - first;
+            const int64_t lens = max(p.lens[lo], 0), at = lens + index;
+            if (at < room) {
+                const int block = static_cast<int>(at >> p.page_shift), held = holds[lo];
+                const int32_t id = block < held ? p.tables[lo * p.table_stride + block] : page_from(lo, block - held);
+                if (id >= 0) slot = (static_cast<int64_t>(id) << p.page_shift) + (at & (page - 1));
+            }
+            position = at;
+            if (p.parents) {
+                position = lens;
+                // each parent comes before its child, so the walk ends; any other number is no parent
+                for (int node = index;;) {
+#pragma unroll
+                    for (int w = 0; w < kMaxWords; ++w)
+                        if (w == node >> 5) bits[w] |= 1u << (node & 31);
+                    const int up = p.parents[first + node];
+                    if (up < 0 || up >= node) break;
+                    node = up;
+                    ++position;
+                }
+            }
+        }
+        p.positions[t] = position;
+        p.slots[t] = slot;
+        if (p.masks)
+#pragma unroll
+            for (int w = 0; w < kMaxWords; ++w)
+                if (w < p.words) p.masks[t * p.words + w] = static_cast<int32_t>(bits[w]);
+    }
+    // the tables' new ends and what the requests hold
+    for (int i = static_cast<int>(thread / 32); i < p.batch; i += static_cast<int>(threads / 32)) {
+        const Need r = need_of(i, starts[i + 1] - starts[i]);
+        const int want = max(r.need - r.held, 0);
+        for (int j = lane; j < want; j += 32) p.tables[i * p.table_stride + r.held + j] = page_from(i, j);
+        __syncwarp();
+        if (lane == 0) {
+            p.held_out[i] = min(r.held, r.need) + min(want, max(there - want_at[i], 0));
+            p.starts[i] = starts[i];
+        }
+    }
+    if (thread == 0) {
+        p.starts[p.batch] = seen;
+        const int64_t left = max(there - pages.b, static_cast<int64_t>(0));
+        p.free_count_out[0] = static_cast<int32_t>(left);
+        p.free_count_out[1] = static_cast<int32_t>(min(pages.b - (there - left) + pages.c, static_cast<int64_t>(0x7fffffff)));
+    }
+}
+
+// ---- the accepted path ------------------------------------------------------------------------------------
+constexpr int kKeepThreads = 128;
+constexpr int kAhead = 8;      // rows read before the first of them is written
+
+struct KeepParams {
+    uint4 *k, *v;
+    const int32_t *tables, *lens, *paths;
+    int32_t *lens_out;
+    int64_t table_stride, path_stride, layer_stride, page_stride, head_stride, row_stride, num_pages;      // strides of the cache in 16-byte vectors
+    int width, page_shift, depth, kv_heads, row_vecs;
+};
+
+// CTA -> (request, layer and cache, part of a token's vectors).  A path ascends, so a row that is moved is never one that an earlier move has overwritten.
+__global__ void __launch_bounds__(kKeepThreads) keep_kernel(const __grid_constant__ KeepParams p) {
+    grid_dependency_sync();
+    const int request = blockIdx.x, layer = blockIdx.y >> 1, vec = blockIdx.z * kKeepThreads + threadIdx.x;
+    uint4 *cache = (blockIdx.y & 1 ? p.v : p.k) + layer * p.layer_stride;
+    const int32_t *path = p.paths + request * p.path_stride, *table = p.tables + request * p.table_stride;
+    const int64_t lens = max(p.lens[request], 0), room = static_cast<int64_t>(p.width) << p.page_shift;
+    const bool mine = vec < p.kv_heads * p.row_vecs;
+    const int64_t inside = mine ? vec / p.row_vecs * p.head_stride + vec % p.row_vecs : 0;
+    // nullptr where there is no such row
+    auto row_of = [&](int64_t token) -> uint4 * {
+        const int64_t at = lens + token;
+        if (!mine || at >= room) return nullptr;
+        const int32_t id = table[at >> p.page_shift];
+        return id < 0 || id >= p.num_pages ? nullptr : cache + id * p.page_stride + (at & ((1 << p.page_shift) - 1)) * p.row_stride + inside;
+    };
+    int last = -1, count = 0;      // of the path so far
+    bool ends = false;
+    for (int base = 0; base < p.depth && !ends; base += kAhead) {
+        uint4 held[kAhead];
+        uint4 *to[kAhead];
+        int node[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) node[j] = base + j < p.depth ? path[base + j] : -1;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            to[j] = nullptr;
+            ends = ends || node[j] <= last;      // the path's end, or no path
+            if (ends) continue;
+            last = node[j];
+            if (node[j] != count) {
+                const uint4 *from = row_of(node[j]);
+                to[j] = row_of(count);
+                if (!from) to[j] = nullptr;
+                else if (to[j]) held[j] = *from;
+            }
+            ++count;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (to[j]) *to[j] = held[j];
+    }
+    if (blockIdx.y == 0 && vec == 0) p.lens_out[request] = static_cast<int32_t>(min(lens + count, static_cast<int64_t>(0x7fffffff)));
+}
+
+int page_shift_of(int page_size) {
+    int s = 0;
+    while ((1 << s) < page_size) ++s;
+    return s;
+}
+bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
+
+}  // namespace
+
+cudaError_t paged_ops_setup() {
+    return cudaFuncSetAttribute(reinterpret_cast<const void *>(&plan_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * kMaxRequests + 1) * 4);
+}
+
+}  // namespace gpuk
+
+using namespace gpuk;
+
+extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int32_t *tables, int64_t table_stride, int table_width, const int32_t *held, int32_t *free_pages,
+                               int free_capacity, const int32_t *free_count, const int32_t *parents, int batch, int total, int page_size, int mask_words, int32_t *starts,
+                               int64_t *positions, int64_t *slots, int32_t *masks, int32_t *held_out, int32_t *free_count_out, void *stream) {
+    if (batch < 0 || total < 0 || table_width < 0 || table_stride < 0 || free_capacity < 0 || mask_words < 0)
+        return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_plan: bad sizes");
+    if (!power_of_two(page_size) || page_size > 65536) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_plan: pages of %d tokens; built for powers of two up to 65536", page_size);
+    if (batch > kMaxRequests) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_plan: %d requests; built for at most %d", batch, kMaxRequests);
+    if (!parents != !masks || (masks && (mask_words < 1 || mask_words > kMaxWords)))
+        return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_plan: parents come with masks of 1 to %d words", kMaxWords);
+    if (static_cast<int64_t>(batch) * table_width > 0x7fffffffll || static_cast<int64_t>(table_width) * page_size > 0x7fffff00ll)
+        return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_plan: tables of %d x %d pages are too large", batch, table_width);
+    if (!starts || !free_count || !free_count_out || (batch && (!lens || !new_lens || !held || !held_out || (table_width && !tables))) || (free_capacity && !free_pages) ||
+        (total && (!positions || !slots)))
+        return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_plan: null pointer");
+    const DecodeDevice *d = nullptr;
+    const int rc = decode_device(&d);
+    if (rc != GPUK_OK) return rc;
+    PlanParams p = {lens, new_lens, held, free_count, parents, tables, free_pages, starts, masks, held_out, free_count_out, positions, slots, table_stride, batch, table_width,
+                    page_shift_of(page_size), free_capacity, total, mask_words};
+    int ctas = 1;
+    while (ctas < 8 && total > ctas * kPlanThreads) ctas *= 2;
+    void *args[] = {&p};
+    const cudaError_t e = launch_kernel(reinterpret_cast<const void *>(&plan_kernel), ctas, kPlanThreads, ctas, false, args, static_cast<cudaStream_t>(stream), (4 * batch + 1) * 4);
+    if (e != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_plan: launch failed: %s", cudaGetErrorString(e));
+    return GPUK_OK;
+}
+
+extern "C" int gpuk_paged_keep(const gpuk_pages *pages, int layers, int64_t layer_stride, const int32_t *tables, int64_t table_stride, int table_width, const int32_t *lens,
+                               const int32_t *paths, int64_t path_stride, int depth, int32_t *lens_out, int batch, void *stream) {
+    if (!pages) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: no pages");
+    if (batch < 0 || layers <= 0 || depth < 0 || table_width < 0 || pages->kv_heads <= 0 || pages->head_dim <= 0 || pages->num_pages < 0)
+        return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: bad sizes");
+    if (pages->dtype != GPUK_DTYPE_BF16 && pages->dtype != GPUK_DTYPE_F16) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_keep: built for bf16 and fp16");
+    if (pages->head_dim % 8 || static_cast<int64_t>(pages->kv_heads) * pages->head_dim > 1 << 24)
+        return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_keep: heads of %d are no multiple of 8, or too many", pages->head_dim);
+    if (!power_of_two(pages->page_size) || pages->page_size > 65536) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_keep: pages of %d tokens; built for powers of two up to 65536", pages->page_size);
+    if (layers > 32767) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_keep: too many layers");
+    if (batch == 0) return GPUK_OK;
+    if (!lens || !lens_out || (depth && !paths) || (table_width && !tables) || !pages->k || !pages->v) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: null pointer");
+    if ((reinterpret_cast<uintptr_t>(pages->k) | reinterpret_cast<uintptr_t>(pages->v)) & 15u) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: pointers must be 16-byte aligned");
+    for (int64_t s : {layer_stride, pages->page_stride, pages->head_stride, pages->row_stride})
+        if (s < 0 || s % 8) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: strides must be multiples of 8 values");
+    KeepParams p = {static_cast<uint4 *>(pages->k), static_cast<uint4 *>(pages->v), tables, lens, paths, lens_out, table_stride, path_stride, layer_stride / 8,
+                    pages->page_stride / 8, pages->head_stride / 8, pages->row_stride / 8, pages->num_pages, table_width, page_shift_of(pages->page_size), depth, pages->kv_heads,
+                    pages->head_dim / 8};
+    // the launch below takes three dimensions
+    const int64_t parts = (static_cast<int64_t>(p.kv_heads) * p.row_vecs + kKeepThreads - 1) / kKeepThreads;
+    if (parts > 65535) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_keep: too many heads");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(batch, 2 * layers, static_cast<unsigned>(parts));
+    cfg.blockDim = dim3(kKeepThreads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    void *args[] = {&p};
+    const cudaError_t e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void *>(&keep_kernel), args);
+    if (e != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_keep: launch failed: %s", cudaGetErrorString(e));
+    return GPUK_OK;
+}

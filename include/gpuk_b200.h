@@ -409,6 +409,69 @@ int gpuk_rope_append(const void *qkv, const float *cos, const float *sin, const 
 int gpuk_silu_mul(const void *in, void *out, int64_t rows, int f, void *stream);
 
 /*
+ * A paged KV cache and what is done with it in a step (no counterpart in the reference, whose caches are one row per sequence,
+ * model/transformer_model.py:674).  Tokens of requests of any lengths lie one after another in [tokens, heads, head_dim]; those of request i are rows
+ * [starts[i], starts[i + 1]).  Its token at position p is in page tables[i][p / page_size] at row p % page_size; slot = page * page_size + row.
+ *
+ * gpuk_pages: one layer's keys and values, [num_pages, kv_heads, page_size, head_dim] in any order of the first three dimensions: strides in values, those
+ * of the two tensors alike, head_dim contiguous.  16-byte aligned, strides multiples of 8.  page_size is a power of two.
+ */
+typedef struct gpuk_pages {
+    void *k, *v;
+    int64_t page_stride, head_stride, row_stride;
+    int64_t num_pages;
+    int kv_heads, page_size, head_dim, dtype;      /* bf16 or fp16 */
+} gpuk_pages;
+/*
+ * The block tables of `batch` requests made to fit lens[i] cached and new_lens[i] new tokens, and a plan of the new ones.  held[i] pages of row i of the table
+ * are in use.  Pages that are too many go on top of the free list (free_pages[0 .. free_count[0])), in order of requests and of pages; pages that are missing
+ * then come from its top in the same order.  tables and free_pages are changed in place, where nothing that the call reads stands: it may be repeated with the
+ * same arguments.  held_out and free_count_out may be held and free_count.  free_count_out[1] is the number of pages that were not to be had (table row or list at its end):
+ * their entries are -1, their tokens have slot -1.
+ *
+ * Out: starts [batch + 1]; for each of `total` rows its position, its slot, and with parents its mask.  parents[t] is the index, in its request, of the token
+ * that t continues: an earlier one; any other number means the cached tokens.  position = lens + index, or with parents lens + the number of ancestors; bit j of a
+ * row's mask (mask_words words of 32) says that new token j is one of its ancestors or itself.  Rows behind the last request have position and slot -1 and
+ * no bits.  New tokens that do not fit `total` are left out.  At most 4096 requests and 8 words.
+ */
+int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int32_t *tables, int64_t table_stride, int table_width, const int32_t *held, int32_t *free_pages,
+                    int free_capacity, const int32_t *free_count, const int32_t *parents, int batch, int total, int page_size, int mask_words, int32_t *starts,
+                    int64_t *positions, int64_t *slots, int32_t *masks, int32_t *held_out, int32_t *free_count_out, void *stream);
+/*
+ * Rotary embedding of the first `rotary` values of each head: pairs (a, b) become (a cos - b sin, b cos + a sin), times amplitude, at the angle
+ * position * turns[i] of a turn (turns: fractions of 2^64, so that far positions lose nothing).  The pairs are (i, i + rotary / 2) (HALF), (2 i, 2 i + 1)
+ * (INTERLEAVED), or (2 i, 2 i + 1) in and (i, i + rotary / 2) out (SPLIT, the order of gpuk_rope_append).  The other values are copied.  head_dim and rotary
+ * multiples of 16, rotary at most 256; bf16 or fp16; strides in values, multiples of 8.  gpuk_rope may work in place, but for SPLIT.
+ *
+ * gpuk_rope_paged rotates queries into q_out and keys into their slots, and copies values into theirs.  A token whose slot is negative or outside the
+ * pages writes nothing to the cache and its queries are NaN; gpuk_fp8_linear_status reports one that is outside.
+ */
+enum { GPUK_ROPE_HALF = 0, GPUK_ROPE_INTERLEAVED = 1, GPUK_ROPE_SPLIT = 2 };
+int gpuk_rope(const void *x, int64_t token_stride, int64_t head_stride, void *out, int64_t out_token_stride, int64_t out_head_stride, const int64_t *positions,
+              const int64_t *turns, float amplitude, int tokens, int heads, int head_dim, int rotary, int layout, int dtype, void *stream);
+int gpuk_rope_paged(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                    int64_t v_token_stride, int64_t v_head_stride, void *q_out, int64_t out_token_stride, int64_t out_head_stride, const int64_t *positions,
+                    const int64_t *slots, const int64_t *turns, float amplitude, const gpuk_pages *pages, int tokens, int heads, int rotary, int layout, void *stream);
+/*
+ * Attention of the new tokens over their requests' pages: softmax(scale * q . k^T) . v in fp32, one rounding.  Their keys and values are in the pages already,
+ * behind lens[i] cached tokens.  A new token sees all cached ones and, of the new ones, those up to itself, or with masks [tokens, mask_words] those whose bit is set
+ * (bit j: new token j of its request).  A row that sees no key is zeros; keys that a row does not see do not reach it, be they infinite or NaN.  Rows of q
+ * behind starts[batch] are not read and those of out not written.  Heads of 64 and 128, up to 128 query heads per kv head, bf16 and fp16, pages of at least 8 tokens.  Pages outside
+ * the pool read as zeros.  max_len: no request has more cached and new tokens (it decides whether keys are split over CTAs, not the result).  q and out: strides
+ * in values, positive multiples of 8, 16-byte aligned.  The workspace belongs to the call until it is done on the stream.
+ */
+int gpuk_paged_attention_workspace(const gpuk_pages *pages, int batch, int tokens, int heads, int64_t max_len, int64_t *bytes);
+int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const gpuk_pages *pages, const int32_t *tables, int64_t table_stride, int table_width,
+                         const int32_t *lens, const int32_t *starts, const int32_t *masks, int mask_words, void *out, int64_t out_token_stride, int64_t out_head_stride,
+                         int batch, int tokens, int heads, int64_t max_len, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+/*
+ * The accepted path of each request's tree: new token path[j] becomes cached token lens + j, in `layers` layers of keys and values.  A path [depth] ascends
+ * strictly from 0 or more and ends at the first entry that does not (-1 by habit).  lens_out[i] = lens[i] + its length; lens_out is not lens.
+ */
+int gpuk_paged_keep(const gpuk_pages *pages, int layers, int64_t layer_stride, const int32_t *tables, int64_t table_stride, int table_width, const int32_t *lens,
+                    const int32_t *paths, int64_t path_stride, int depth, int32_t *lens_out, int batch, void *stream);
+
+/*
  * No counterpart in the reference.  Same job as gpuk_emulated_allreduce_rms (fused op only)
  * for callers that must not allocate device memory -- a health probe or test harness inside a
  * process whose own arena already owns the GPU's memory, where a library-side cudaMalloc may
