@@ -58,11 +58,13 @@ struct alignas(16) Unit {                        // what a CTA of the first kern
     int found;
 };
 
+// A wait tells a phase of a barrier from the one before and the one behind it, not from the next but one.  Scores and products have two barriers in turn, since a row's thread may
+// come to block j when product j - 2 is the last that is known to be complete, and to its end when the last product is.
 template <int HD>
 struct Smem {
     alignas(1024) unsigned char q[HD / 64 * kQSpanBytes];
     alignas(1024) unsigned char ring[kSlotsOf<HD>][HD / 64 * kSpanBytes];
-    uint64_t q_full, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done, drained;
+    uint64_t q_full, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done[2], drained;
     Unit unit;
     uint32_t tmem;
     uint32_t poison[kMaskedBlocks * 2];          // keys of the masked blocks with a value that is no finite number
@@ -96,7 +98,7 @@ template <>
 struct Half<__nv_bfloat16> {
     static constexpr int kFormat = 1;
     static constexpr uint32_t kExponent = 0x7f807f80u;
-    static constexpr float kBias = 0.f;
+    static constexpr float kBias = 0.f, kLag = 8.f;
     __device__ static uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -107,7 +109,7 @@ template <>
 struct Half<__half> {
     static constexpr int kFormat = 0;
     static constexpr uint32_t kExponent = 0x7c007c00u;
-    static constexpr float kBias = 10.f;
+    static constexpr float kBias = 8.f, kLag = 7.f;      // 2^15 at most
     __device__ static uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -255,9 +257,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) find_unit(p, &sm.unit, blockIdx.x);
     if (tid == kRows) {
-        mbar_init(&sm.q_full, 1), mbar_init(&sm.o_done, 1), mbar_init(&sm.drained, 1);
+        mbar_init(&sm.q_full, 1), mbar_init(&sm.drained, 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-        for (int b = 0; b < 2; ++b) mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows);
+        for (int b = 0; b < 2; ++b) mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows), mbar_init(&sm.o_done[b], 1);
         mbar_init_fence();
     }
     if (tid >= kRows + 32 && tid < kRows + 32 + kMaskedBlocks * 2) sm.poison[tid - kRows - 32] = 0;
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
                     tc_mma_f16_ts(tm + kOut, tm + (j & 1) * kKeys + k * 8, mnmajor_desc(v + k * 16 * 128, kSpanBytes), o_desc, j > 0 || k > 0);
-                tc_commit(&sm.o_done);
+                tc_commit(&sm.o_done[j & 1]);
                 release(v_at(j));
             }
             if (!ok) {      // a wait gave up: the row threads do not wait for what was issued, and the tensor memory is about to be freed
@@ -429,11 +431,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                 }
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
                 if (some) top = fmaxf(top, kSeen);
-                const bool grown = top > m;
+                const bool grown = top > m + Half<T>::kLag;
                 if (j == 0) {
                     m = fmaxf(top, kLowest);
                 } else if (__any_sync(0xffffffffu, grown)) {
-                    ok = mbar_wait(&sm.o_done, (j - 1) & 1) && ok;
+                    ok = mbar_wait(&sm.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1) && ok;
                     __syncwarp();
                     tc_fence_after();
                     const float f = grown ? exp2_fast(m - top) : 1.f;
@@ -466,9 +468,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             mbar_arrive(&sm.p_full[j & 1]);
         }
         if (blocks > 0 && ok) {
-            // the scores of the last block are ready before the product of the one before it is: one phase after the other, since a wait cannot tell a phase from the next but one
-            if (blocks > 1) ok = mbar_wait(&sm.o_done, (blocks - 2) & 1);
-            ok = mbar_wait(&sm.o_done, (blocks - 1) & 1) && ok;
+            ok = mbar_wait(&sm.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1) && ok;
             tc_fence_after();
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
