@@ -41,8 +41,11 @@ constexpr int kQSpanBytes = kRows * 128;
 constexpr int kColumns = 256;                    // two score buffers of 64, up to 128 of outputs
 constexpr int kOut = 2 * kKeys;                  // first column of the outputs
 constexpr int kMaskedBlocks = 8;                 // that a tile can have
-constexpr int kMinPart = 4;                      // blocks of a part
 constexpr int kCtasPerSm = 2;
+constexpr int kTileCost = 4 * kKeys;             // what a tile costs beside its keys, in keys: its queries, its outputs, the first scores
+constexpr int kGrain = kTileCost + 2 * kKeys;    // no tile is cut nearer than that to one of its ends
+constexpr int kPerCta = 256;                     // keys for which a call takes another CTA
+constexpr int kQueue = 4;                        // segments that are described at a time
 
 constexpr float kLowest = -3.4e38f;              // a maximum before any key ...
 constexpr float kSeen = -3.3e38f;                // ... and where all scores are -infinity: finite both, and below any score behind them
@@ -50,24 +53,35 @@ constexpr float kSeen = -3.3e38f;                // ... and where all scores are
 template <int HD>
 constexpr int kSlotsOf = HD == 128 ? 5 : 10;
 
-struct alignas(16) Unit {                        // what a CTA of the first kernel does, or a joined tile
+// Blocks [first, first + blocks) of the keys of a tile: what a CTA does at a time.
+struct alignas(16) Segment {
     int request, start, n, ctx;                  // its first row in q, new and cached tokens
-    int tile, kvh;
-    int part, parts, first, last;                // blocks [first, last)
-    int slot;                                    // of the partial results, where there are parts
-    int found;
+    int tok0, kvh;                               // the tile's first token
+    int first, blocks;                           // no blocks: the end
+    int slot;                                    // of the partial results; -1: the whole tile
+};
+struct Request {
+    int start, n, ctx, tiles;
+    bool over;      // more tokens than the table's row holds: its tiles are not cut
+};
+// Where a CTA begins: weight `pos` of a tile; and its borders on the line of all tiles.
+struct Start {
+    Request r;
+    int request, kvh, tile, ctas;
+    int64_t pos, x[2];
 };
 
-// A wait tells a phase of a barrier from the one before and the one behind it, not from the next but one.  Scores and products have two barriers in turn, since a row's thread may
-// come to block j when product j - 2 is the last that is known to be complete, and to its end when the last product is.
+// A wait tells a phase of a barrier from the one before and the one behind it, not from the next but one.  Scores, products and queries have two barriers in turn, since a row's thread
+// may come to block j when product j - 2 is the last that is known to be complete, and to its end when the last product is.
 template <int HD>
 struct Smem {
     alignas(1024) unsigned char q[HD / 64 * kQSpanBytes];
     alignas(1024) unsigned char ring[kSlotsOf<HD>][HD / 64 * kSpanBytes];
-    uint64_t q_full, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done[2], drained;
-    Unit unit;
+    uint64_t q_full[2], q_empty, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done[2], drained;
+    Segment queue[kQueue];
+    Start start;
     uint32_t tmem;
-    uint32_t poison[kMaskedBlocks * 2];          // keys of the masked blocks with a value that is no finite number
+    uint32_t poison[3][kMaskedBlocks * 2];       // keys of the masked blocks with a value that is no finite number, of a segment, the next and the one before
 };
 
 struct PagedAttentionParams {
@@ -77,14 +91,20 @@ struct PagedAttentionParams {
     int64_t table_stride, page_stride, head_stride, row_stride, num_pages;
     int64_t out_token, out_head;
     int batch, tokens, kv_heads, group, tile_tokens, words;
+    uint32_t tile_inverse;                       // 2^32 / tile_tokens, rounded up
     int width, page_shift;                       // of a row of the table, and log2 of a page's tokens
-    int target;                                  // CTAs that run at once
-    int may_split;
+    int may_split, out_sectors;                  // rows of the outputs lie on borders of 32 bytes
     float scale_log2;
     int *status;
-    int *units;                                  // count, then a Unit of each tile that is joined
-    float *partial;                              // [slot][128][HD], [slot][2][128]: outputs, then maxima and sums
-    int max_slots;
+    // of the partial results, for `ctas` CTAs: see Joint, [2 * ctas][HD / 4][128][4] outputs (a warp's rows side by side), [2 * ctas][2][128] maxima and sums
+    struct Joint *joints;
+    float *partial, *stats;
+};
+// What the second kernel learns from each CTA of the first.
+struct alignas(16) Joint {
+    Segment open;                                // a tile that begins in the CTA and goes on behind it (slot -1: none)
+    int head;                                    // the CTA takes: 0 nothing, 1 a part of such a tile and nothing else, 2 the last part of one, 3 begins with a tile
+    int ctas;                                    // that take part
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -116,118 +136,161 @@ struct Half<__half> {
         return r;
     }
 };
-// Whether one of the two halves is an infinity or NaN: all bits of its exponent are set.
-__device__ __forceinline__ bool any_not_finite(uint32_t w, uint32_t exponent) {
+// Nonzero where one of the two halves is an infinity or NaN: all bits of its exponent are set.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w, uint32_t exponent) {
     const uint32_t x = (w & exponent) ^ exponent;      // a zero half
-    return ((x - 0x00010001u) & ~x & 0x80008000u) != 0;
+    return (x - 0x00010001u) & ~x & 0x80008000u;
+}
+// 32 bytes, a whole sector: a warp's rows lie apart, and each store of theirs is a sector a row.
+__device__ __forceinline__ void store_sector(void *to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
-// ---- which part of which tile a CTA takes ---------------------------------------------------------
-struct Request {
-    int start, n, ctx, tiles, blocks;
-};
+// Barriers by their address in shared memory: the single threads that copy and multiply are bound by the instructions between two waits.
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity) {
+    for (uint32_t spin = 0; spin < (1u << 24); ++spin) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void commit_at(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// One lane of a warp that is together.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// ---- which parts of which tiles a CTA takes ---------------------------------------------------------
+// Tiles lie one after another, by request, kv head and token, each as long as the keys that it sees and kTileCost more.  A CTA takes an equal share of that line; where a border comes
+// near an end of a tile it goes to that end.
+__device__ __forceinline__ int64_t room_of(const PagedAttentionParams &p) { return static_cast<int64_t>(p.width) << p.page_shift; }
 __device__ __forceinline__ Request request_of(const PagedAttentionParams &p, int i) {
     Request r;
     r.start = min(max(p.starts[i], 0), p.tokens);
     r.n = min(max(p.starts[i + 1], r.start), p.tokens) - r.start;
-    const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;      // what the row of the table can hold
-    r.ctx = static_cast<int>(min(static_cast<int64_t>(max(p.lens[i], 0)), room));
-    const int64_t end = min(static_cast<int64_t>(r.ctx) + r.n, room);
-    r.tiles = (r.n + p.tile_tokens - 1) / p.tile_tokens;
-    r.blocks = static_cast<int>((end + kKeys - 1) / kKeys);
+    r.ctx = static_cast<int>(min(static_cast<int64_t>(max(p.lens[i], 0)), room_of(p)));
+    r.tiles = static_cast<int>(p.tile_tokens == 1 ? r.n : __umulhi(r.n + p.tile_tokens - 1, p.tile_inverse));      // exact below 2^32 / tile_tokens
+    r.over = static_cast<int64_t>(r.ctx) + r.n > room_of(p);
     return r;
 }
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+// Keys that some row of a tile sees.
+__device__ __forceinline__ int64_t keys_of(const PagedAttentionParams &p, const Request &r, int tile) {
+    const int64_t most = static_cast<int64_t>(r.ctx) + (p.masks ? static_cast<int64_t>(r.n) : min(static_cast<int64_t>(r.n), static_cast<int64_t>(tile + 1) * p.tile_tokens));
+    return min(most, room_of(p));
 }
-__device__ __forceinline__ int64_t warp_before(int64_t v, int lane) {
-    int64_t s = v;
+// The weight of the tiles in front of one.
+__device__ __forceinline__ int64_t weight_before(const PagedAttentionParams &p, const Request &r, int tile) {
+    if (r.tiles == 0) return 0;
+    if (p.masks || r.over) return tile * (kTileCost + min(static_cast<int64_t>(r.ctx) + r.n, room_of(p)));
+    const int64_t whole = min(tile, r.tiles - 1), w = whole * (kTileCost + r.ctx) + p.tile_tokens * (whole * (whole + 1) / 2);
+    return tile < r.tiles || tile == 0 ? w : w + kTileCost + r.ctx + r.n;
+}
+// Sums over the lanes up to this one.
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
+        const int64_t t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
     }
-    return s - v;
+    return v;
 }
 
-// One warp.  Lane l looks after a run of the requests; parts of `cut` blocks, the fewest with which all parts run at once.
-__device__ void find_unit(const PagedAttentionParams &p, Unit *u, int item) {
+// One warp for each of a CTA's two borders; lane l looks after a run of the requests.  Quotients are estimated in fp32 and put right, which is faster than dividing 64 bits.
+__device__ void find_border(const PagedAttentionParams &p, Start *out, int side) {
     const int lane = threadIdx.x & 31, per = (p.batch + 31) / 32, lo = min(lane * per, p.batch), hi = min(lo + per, p.batch);
-    const int kvh = item % p.kv_heads, rest = item / p.kv_heads;
-    int cut = 1 << 30;
-    if (p.may_split) {
-        int64_t work = 0;
-        int most = 0;
-        for (int i = lo; i < hi; ++i) {
-            const Request r = request_of(p, i);
-            work += static_cast<int64_t>(r.tiles) * r.blocks;
-            if (r.tiles) most = max(most, r.blocks);
-        }
-        work = warp_sum(work) * p.kv_heads;
-        most = __reduce_max_sync(0xffffffffu, most);
-        cut = static_cast<int>(max(static_cast<int64_t>(kMinPart), (work + p.target - 1) / p.target));
-        for (int tries = 0; tries < 6 && cut < most; ++tries) {
-            int64_t items = 0;
-            for (int i = lo; i < hi; ++i) {
-                const Request r = request_of(p, i);
-                items += static_cast<int64_t>(r.tiles) * ((r.blocks + cut - 1) / cut);
-            }
-            if (warp_sum(items) * p.kv_heads <= p.target) break;
-            cut += cut / 4 + 1;
-        }
-    }
-    int64_t items = 0, joined = 0, tiles = 0;      // of this lane's requests: CTAs per kv head, those of tiles in parts, such tiles
+    int64_t weight = 0, tiles = 0;
+    Request r = {};
     for (int i = lo; i < hi; ++i) {
-        const Request r = request_of(p, i);
-        const int parts = max(1, (r.blocks + cut - 1) / cut);
-        items += static_cast<int64_t>(r.tiles) * parts;
-        if (parts > 1) joined += static_cast<int64_t>(r.tiles) * parts, tiles += r.tiles;
+        r = request_of(p, i);
+        weight += weight_before(p, r, r.tiles) * p.kv_heads, tiles += static_cast<int64_t>(r.tiles) * p.kv_heads;
     }
-    int64_t before = warp_before(items, lane), joined_before = warp_before(joined, lane), tiles_before = warp_before(tiles, lane);
-    if (p.may_split && item == 0) {
-        const int64_t all = warp_sum(tiles) * p.kv_heads;
-        if (lane == 0) p.units[0] = static_cast<int>(all);
+    const int64_t upto = warp_scan(weight, lane), all = __shfl_sync(0xffffffffu, upto, 31), before = upto - weight;
+    // enough borders for each tile to have a CTA of its own where there are few
+    const int few = __reduce_add_sync(0xffffffffu, static_cast<int>(min(tiles, static_cast<int64_t>(1 << 20))));
+    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), 2 * few + all / kPerCta));
+    const int border = static_cast<int>(blockIdx.x) + side;
+    const int64_t raw = border < ctas ? static_cast<int64_t>(static_cast<double>(all) / ctas * border) : all;
+    if (raw >= all) {      // the line's end
+        if (lane == 0) out->x[side] = all, out->ctas = ctas;
+        return;
     }
-    const bool mine = rest >= before && rest < before + items;
-    if (lane == 0) u->found = 0;
-    __syncwarp();
-    if (!mine) return;
+    if (raw < before || raw >= upto) return;
+    int64_t base = before;
     for (int i = lo; i < hi; ++i) {
-        const Request r = request_of(p, i);
-        const int parts = max(1, (r.blocks + cut - 1) / cut);
-        const int64_t here = static_cast<int64_t>(r.tiles) * parts;
-        if (rest < before + here) {
-            const int at = static_cast<int>(rest - before);
-            Unit v;
-            v.request = i, v.start = r.start, v.n = r.n, v.ctx = r.ctx, v.kvh = kvh;
-            v.tile = r.tiles - 1 - at / parts;      // the tiles that see most come first
-            v.part = at % parts, v.parts = parts;
-            // keys that some row of the tile sees
-            const int64_t end = min(static_cast<int64_t>(r.ctx) + (p.masks ? r.n : min(r.n, (v.tile + 1) * p.tile_tokens)), static_cast<int64_t>(p.width) << p.page_shift);
-            const int blocks = static_cast<int>((end + kKeys - 1) / kKeys);
-            v.first = static_cast<int>(min(static_cast<int64_t>(v.part) * cut, static_cast<int64_t>(blocks)));
-            v.last = static_cast<int>(min(static_cast<int64_t>(v.first) + cut, static_cast<int64_t>(blocks)));
-            v.slot = 0;
-            v.found = 1;
-            if (parts > 1) {
-                const int64_t tile = (tiles_before + v.tile) * p.kv_heads + kvh;
-                const int64_t slot = joined_before * p.kv_heads + (static_cast<int64_t>(v.tile) * p.kv_heads + kvh) * parts + v.part;
-                if (slot - v.part + parts > p.max_slots || tile >= p.target) {      // cannot be: the parts of joined tiles are at most twice the target
-                    *p.status = 1;
-                    v.found = 0;
-                }
-                v.slot = static_cast<int>(slot);
-                if (v.part == 0 && v.found) reinterpret_cast<Unit *>(p.units + 4)[tile] = v;
-            }
-            *u = v;
-            return;
+        if (per > 1) r = request_of(p, i);
+        const int64_t head = weight_before(p, r, r.tiles), here = head * p.kv_heads;
+        if (raw >= base + here) {
+            base += here;
+            continue;
         }
-        before += here;
-        if (parts > 1) joined_before += here, tiles_before += r.tiles;
+        int64_t at = raw - base;
+        int kvh = min(p.kv_heads - 1, static_cast<int>(__fdividef(static_cast<float>(at), static_cast<float>(head))));
+        while (kvh > 0 && kvh * head > at) --kvh;
+        while (kvh + 1 < p.kv_heads && (kvh + 1) * head <= at) ++kvh;
+        at -= kvh * head;
+        // weight_before(tile) <= at < weight_before(tile + 1): a line, or a parabola with half a tile's tokens to the square
+        const float slope = kTileCost + r.ctx + (p.masks || r.over ? static_cast<float>(r.n) : 0.5f * p.tile_tokens), bend = p.masks || r.over ? 0.f : 0.5f * p.tile_tokens;
+        int tile = min(r.tiles - 1, static_cast<int>(bend == 0.f ? static_cast<float>(at) / slope : (sqrtf(slope * slope + 4.f * bend * at) - slope) / (2.f * bend)));
+        while (tile > 0 && weight_before(p, r, tile) > at) --tile;
+        while (tile + 1 < r.tiles && weight_before(p, r, tile + 1) <= at) ++tile;
+        const int64_t first = weight_before(p, r, tile), size = weight_before(p, r, tile + 1) - first;
+        int64_t pos = at - first;
+        if (!p.may_split || r.over || pos < kGrain) pos = 0;
+        else if (size - pos < kGrain) pos = size;
+        else pos = pos / kKeys * kKeys;      // the borders of blocks, behind the tile's cost
+        out->x[side] = base + kvh * head + first + pos, out->ctas = ctas;
+        if (side == 0) out->r = r, out->request = i, out->kvh = kvh, out->tile = tile, out->pos = pos;
+        return;
     }
 }
+
+// The segments of a CTA one after another.
+struct Walk {
+    Request r;
+    int request, kvh, tile, index;
+    int64_t pos, left;
+    __device__ explicit Walk(const Start &s) : r(s.r), request(s.request), kvh(s.kvh), tile(s.tile), index(0), pos(s.pos), left(s.x[1] - s.x[0]) {}
+    __device__ bool next(const PagedAttentionParams &p, Segment *out, bool *begins, bool *ends) {
+        if (left <= 0) return false;
+        int64_t size = weight_before(p, r, tile + 1) - weight_before(p, r, tile);
+        while (pos >= size) {      // at a tile's end, to the next
+            pos = 0;
+            if (++tile >= r.tiles) {
+                tile = 0;
+                if (++kvh >= p.kv_heads) {
+                    kvh = 0;
+                    do {
+                        if (++request >= p.batch) return false;      // cannot be: the weights say that there is more
+                        r = request_of(p, request);
+                    } while (r.tiles == 0);
+                }
+            }
+            size = weight_before(p, r, tile + 1) - weight_before(p, r, tile);
+        }
+        const int64_t take = min(size - pos, left), end = pos + take;
+        const int all = static_cast<int>((keys_of(p, r, tile) + kKeys - 1) / kKeys);
+        auto block_at = [&](int64_t w) { return w <= kTileCost ? 0 : static_cast<int>(min((w - kTileCost + kKeys - 1) / kKeys, static_cast<int64_t>(all))); };
+        *begins = pos == 0, *ends = end == size;
+        const int first = *begins ? 0 : block_at(pos), last = *ends ? all : block_at(end);
+        *out = {request, r.start, r.n, r.ctx, tile * p.tile_tokens, kvh, first, last - first, -1};
+        if (!*begins || !*ends) out->slot = 2 * static_cast<int>(blockIdx.x) + (*begins && index > 0);
+        pos = end, left -= take, ++index;
+        return true;
+    }
+};
 
 // Bits [at, at + 64) of a row of mask words, zeros outside.
 __device__ __forceinline__ uint64_t mask_bits(const int32_t *row, int words, int at) {
@@ -236,7 +299,7 @@ __device__ __forceinline__ uint64_t mask_bits(const int32_t *row, int words, int
     return static_cast<uint64_t>(__funnelshift_r(a, b, s)) | static_cast<uint64_t>(__funnelshift_r(b, c, s)) << 32;
 }
 // Which keys of block `base` a row sees: cached ones, and of the new ones those up to token `tok` or those in its mask.
-__device__ __forceinline__ uint64_t seen_of(const PagedAttentionParams &p, const Unit &u, int tok, int base) {
+__device__ __forceinline__ uint64_t seen_of(const PagedAttentionParams &p, const Segment &u, int tok, int base) {
     const int old = min(max(u.ctx - base, 0), kKeys);      // keys of the block in front of the new ones
     const uint64_t cached = old == kKeys ? ~0ull : (1ull << old) - 1;
     if (old == kKeys) return cached;
@@ -254,275 +317,350 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     extern __shared__ __align__(1024) unsigned char dyn[];
     Smem<HD> &sm = *reinterpret_cast<Smem<HD> *>(dyn);
     const int tid = threadIdx.x, warp = tid >> 5;
+    if (tid == kRows + 32) prefetch_map(&qmap), prefetch_map(&kmap), prefetch_map(&vmap);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 0) find_unit(p, &sm.unit, blockIdx.x);
+    if (warp < 2) find_border(p, &sm.start, warp);
     if (tid == kRows) {
-        mbar_init(&sm.q_full, 1), mbar_init(&sm.drained, 1);
+        for (int b = 0; b < 2; ++b) mbar_init(&sm.q_full[b], 1), mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows / 32), mbar_init(&sm.o_done[b], 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-        for (int b = 0; b < 2; ++b) mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows), mbar_init(&sm.o_done[b], 1);
+        mbar_init(&sm.q_empty, 1), mbar_init(&sm.drained, 1);
         mbar_init_fence();
     }
-    if (tid >= kRows + 32 && tid < kRows + 32 + kMaskedBlocks * 2) sm.poison[tid - kRows - 32] = 0;
+    if (tid >= kRows + 32)
+        for (int i = tid - kRows - 32; i < 3 * kMaskedBlocks * 2; i += 32) sm.poison[0][i] = 0;
     __syncthreads();
-    const Unit u = sm.unit;
-    if (!u.found) return;
+    if (sm.start.x[1] <= sm.start.x[0]) {      // a border that went to an end of its tile, or fewer CTAs than there are
+        if (tid == 0 && p.may_split) p.joints[blockIdx.x].open.slot = -1, p.joints[blockIdx.x].head = 0, p.joints[blockIdx.x].ctas = sm.start.ctas;
+        return;
+    }
     if (warp == kRows / 32) tmem_alloc<kColumns>(&sm.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // behind the allocation: no CTA that follows takes columns one of this grid waits for
     const uint32_t tm = sm.tmem;
-    const int blocks = u.last - u.first, tok0 = u.tile * p.tile_tokens;
-    // keys from here on are not seen by every row, or are no keys
-    const int64_t limit = p.masks ? u.ctx : static_cast<int64_t>(u.ctx) + tok0 + 1;
-    const int first_masked = max(u.first, static_cast<int>(limit / kKeys));
     bool ok = (smem_addr(dyn) & 1023u) == 0;
 
-    if (warp == kRows / 32 + 1) {      // copies: Q, then K of the first block, and K of the next block before V of each
+    const uint32_t full = smem_addr(sm.full), empty = smem_addr(sm.empty), q_full = smem_addr(sm.q_full), s_full = smem_addr(sm.s_full), p_full = smem_addr(sm.p_full),
+                   o_done = smem_addr(sm.o_done), q_empty = smem_addr(&sm.q_empty);
+
+    if (warp == kRows / 32 + 1) {      // copies: of a segment K of the first block, Q, and K of the next block before V of each
         const int lane = tid & 31;
-        if (ok && blocks > 0) {
-            const uint64_t once = policy_evict_first();
-            if (lane == 0) {
-                mbar_expect_bytes(&sm.q_full, kSpans * p.tile_tokens * p.group * 128);
-                for (int h = 0; h < kSpans; ++h) tma_load_3d(smem_addr(sm.q) + h * kQSpanBytes, &qmap, h * 64, u.kvh * p.group, u.start + tok0, &sm.q_full);
-            }
-            const int rows = min(1 << p.page_shift, kKeys), boxes = kKeys / rows;
+        const int rows = min(1 << p.page_shift, kKeys), box_shift = min(p.page_shift, 6), boxes = kKeys >> box_shift, batch_blocks = 32 >> (6 - box_shift);
+        Walk walk(sm.start);
+        Joint joint;
+        joint.open.slot = -1, joint.head = 3, joint.ctas = sm.start.ctas;
+        int segments = 0, slot = 0, filled = 0;
+        uint32_t phase = 1;      // a fresh slot counts as released
+        Segment u;
+        bool begins, ends;
+        while (ok && walk.next(p, &u, &begins, &ends)) {
+            if (!begins) joint.head = ends ? 2 : 1;
+            if (begins && !ends) joint.open = u;
             const int32_t *table = p.tables + u.request * p.table_stride;
-            // the page of this lane's box in block j; one outside the pool, which reads as zeros, where there is none
-            auto page_of = [&](int j) {
-                const int64_t key = static_cast<int64_t>(u.first + j) * kKeys + lane * rows;
-                const int64_t end = static_cast<int64_t>(u.ctx) + u.n;
-                return lane < boxes && j < blocks && key < end && (key >> p.page_shift) < p.width ? table[key >> p.page_shift] : -1;
+            // Pages by 32 boxes, a lane for each, and the next 32 on their way; one outside the pool, which reads as zeros, where there is none.
+            const int end = static_cast<int>(min(min(static_cast<int64_t>(u.ctx) + u.n, room_of(p)), (static_cast<int64_t>(u.first) + u.blocks) * kKeys));
+            auto pages_from = [&](int j) {
+                const int64_t key = (static_cast<int64_t>(u.first) + j) * kKeys + (lane << box_shift);
+                return key < end ? table[key >> p.page_shift] : -1;
             };
-            int page_k = page_of(0), page_next = page_of(1), page_v = page_k;
-            int filled = 0;
+            int pages = pages_from(0), pages_next = batch_blocks < u.blocks ? pages_from(batch_blocks) : -1, left = batch_blocks, from = 0;
+            const int inside_mask = rows == kKeys ? (1 << p.page_shift) - 1 : 0;
             auto load = [&](const CUtensorMap *map, int j, int page) {
-                const int s = filled % kSlots;
-                if (!mbar_wait(&sm.empty[s], ((filled / kSlots) & 1) ^ 1)) return false;
-                if (lane == 0) mbar_expect_bytes(&sm.full[s], kBlockBytes);
+                const uint32_t bar = full + 8 * slot;
+                if (!wait_at(empty + 8 * slot, phase)) return false;
+                if (lane == 0) expect_at(bar, kBlockBytes);
                 __syncwarp();
                 if (lane < boxes) {
-                    const int inside = (u.first + j) * kKeys & ((1 << p.page_shift) - 1);
-                    for (int h = 0; h < kSpans; ++h)
-                        tma_load_4d(smem_addr(sm.ring[s]) + h * kSpanBytes + lane * rows * 128, map, h * 64, rows == kKeys ? inside : 0, u.kvh, page, &sm.full[s], once);
+                    const int inside = (u.first + j) * kKeys & inside_mask;
+                    const uint32_t to = smem_addr(sm.ring) + slot * kBlockBytes + (lane << box_shift) * 128;
+#pragma unroll
+                    for (int h = 0; h < kSpans; ++h) tma_load_4d(to + h * kSpanBytes, map, h * 64, inside, u.kvh, page, &sm.full[slot]);
                 }
                 ++filled;
+                if (++slot == kSlots) slot = 0, phase ^= 1u;
                 return true;
             };
+            // the pages of the next block
+            auto next_page = [&](int j) {
+                if (left == 0) {
+                    pages = pages_next, left = batch_blocks, from = 0;
+                    pages_next = j + batch_blocks < u.blocks ? pages_from(j + batch_blocks) : -1;
+                }
+                const int page = __shfl_sync(0xffffffffu, pages, (from + lane) & 31);
+                from += boxes, --left;
+                return page;
+            };
+            int page_k = next_page(0);
             ok = load(&kmap, 0, page_k);
-            for (int j = 0; ok && j < blocks; ++j) {
-                page_v = page_k, page_k = page_next, page_next = page_of(j + 2);
-                if (j + 1 < blocks) ok = load(&kmap, j + 1, page_k);
+            if (ok && segments > 0) ok = wait_at(q_empty, (segments - 1) & 1);
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t bar = q_full + 8 * (segments & 1);
+                sm.queue[segments % kQueue] = u;
+                expect_at(bar, kSpans * p.tile_tokens * p.group * 128);
+#pragma unroll
+                for (int h = 0; h < kSpans; ++h) tma_load_3d(smem_addr(sm.q) + h * kQSpanBytes, &qmap, h * 64, u.kvh * p.group, u.start + u.tok0, &sm.q_full[segments & 1]);
+            }
+            ++segments;
+            for (int j = 0; ok && j < u.blocks; ++j) {
+                const int page_v = page_k;
+                if (j + 1 < u.blocks) {
+                    page_k = next_page(j + 1);
+                    ok = load(&kmap, j + 1, page_k);
+                }
                 if (ok) ok = load(&vmap, j, page_v);
             }
-            // nobody leaves with copies in flight
-            ok = mbar_wait(&sm.q_full, 0) && ok;
-            for (int i = max(0, filled - kSlots); i < filled; ++i) ok = mbar_wait(&sm.full[i % kSlots], (i / kSlots) & 1) && ok;
         }
-    } else if (warp == kRows / 32) {   // multiplications
-        if ((tid & 31) == 0 && ok && blocks > 0) {
-            constexpr uint32_t s_desc = mma_desc(Half<T>::kFormat, Half<T>::kFormat, kRows, kKeys), o_desc = mma_desc(Half<T>::kFormat, Half<T>::kFormat, kRows, HD, true);
-            const int loads = 2 * blocks;
-            auto k_at = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
-            auto v_at = [&](int j) { return j + 1 < blocks ? 2 * j + 2 : loads - 1; };
-            auto slot = [&](int i) { return smem_addr(sm.ring[i % kSlots]); };
-            auto wait_slot = [&](int i) { return mbar_wait(&sm.full[i % kSlots], (i / kSlots) & 1); };
-            // only a slot that the copies wait for: nothing may arrive in shared memory behind the CTA's end
-            auto release = [&](int i) {
-                if (i + kSlots < loads) tc_commit(&sm.empty[i % kSlots]);
-            };
-            auto scores = [&](int j) {
-                const uint32_t q = smem_addr(sm.q), k = slot(k_at(j));
+        if (lane == 0 && p.may_split) p.joints[blockIdx.x] = joint;
+        // the end, behind the last segment's scores; and nobody leaves with copies in flight or releases to come
+        if (ok && segments > 0) ok = wait_at(q_empty, (segments - 1) & 1);
+        if (ok && lane == 0) {
+            sm.queue[segments % kQueue].blocks = 0;
+            arrive_at(q_full + 8 * (segments & 1));
+        }
+        if (!ok && segments > 0) wait_at(q_full + 8 * ((segments - 1) & 1), ((segments - 1) >> 1) & 1);
+        for (int i = max(0, filled - kSlots); i < filled; ++i) ok = wait_at((ok ? empty : full) + 8 * (i % kSlots), (i / kSlots) & 1) && ok;
+    } else if (warp == kRows / 32) {   // multiplications: K and V of the ring are used in the order in which they were copied
+        // The whole warp goes through the loop and one lane issues, so that descriptors stay in uniform registers: a lane on its own took 80 cycles an instruction.
+        constexpr uint32_t s_desc = mma_desc(Half<T>::kFormat, Half<T>::kFormat, kRows, kKeys), o_desc = mma_desc(Half<T>::kFormat, Half<T>::kFormat, kRows, HD, true);
+        const uint64_t q_at = kmajor_desc<128>(smem_addr(sm.q)), k_at = kmajor_desc<128>(smem_addr(sm.ring)), v_at = mnmajor_desc(smem_addr(sm.ring), kSpanBytes);
+        const uint32_t out_at = __shfl_sync(0xffffffffu, tm, 0) + kOut, scores_at = out_at - kOut;
+        ok = __all_sync(0xffffffffu, ok);
+        int slot = 0;
+        uint32_t phase = 0, t = 0;      // of the ring; blocks so far
+        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_at(bar, parity)) != 0; };
+        auto taken = [&]() {
+            if (++slot == kSlots) slot = 0, phase ^= 1u;
+        };
+        auto scores = [&](uint32_t t, bool last) {
+            const uint64_t k = k_at + slot * (kBlockBytes / 16);
+            const uint32_t to = scores_at + (t & 1) * kKeys;
+            if (elect_one()) {
 #pragma unroll
-                for (int d = 0; d < HD / 16; ++d)
-                    tc_mma_f16(tm + (j & 1) * kKeys, kmajor_desc<128>(q + (d / 4) * kQSpanBytes + (d % 4) * 32), kmajor_desc<128>(k + (d / 4) * kSpanBytes + (d % 4) * 32), s_desc,
-                               d > 0);
-                tc_commit(&sm.s_full[j & 1]);
-                release(k_at(j));
-            };
-            ok = mbar_wait(&sm.q_full, 0) && wait_slot(0);
+                for (int d = 0; d < HD / 16; ++d) tc_mma_f16(to, q_at + ((d / 4) * kQSpanBytes + (d % 4) * 32) / 16, k + ((d / 4) * kSpanBytes + (d % 4) * 32) / 16, s_desc, d > 0);
+                commit_at(s_full + 8 * (t & 1));
+                commit_at(empty + 8 * slot);
+                if (last) commit_at(q_empty);
+            }
+            taken();
+        };
+        for (uint32_t segment = 0; ok; ++segment) {
+            ok = wait(q_full + 8 * (segment & 1), (segment >> 1) & 1);
+            if (!ok) break;
+            const int blocks = __shfl_sync(0xffffffffu, sm.queue[segment % kQueue].blocks, 0);
+            if (blocks == 0) break;
+            ok = wait(full + 8 * slot, phase);
             tc_fence_after();
-            if (ok) scores(0);
-            for (int j = 0; ok && j < blocks; ++j) {
+            if (ok) scores(t, blocks == 1);
+            for (int j = 0; ok && j < blocks; ++j, ++t) {
                 if (j + 1 < blocks) {
-                    ok = wait_slot(k_at(j + 1));
+                    ok = wait(full + 8 * slot, phase);
                     tc_fence_after();
                     if (!ok) break;
-                    scores(j + 1);      // into the buffer of P(j - 1), whose product is in front of it
+                    scores(t + 1, j + 2 == blocks);      // into the buffer of P(t - 1), whose product is in front of it
                 }
-                ok = wait_slot(v_at(j)) && mbar_wait(&sm.p_full[j & 1], (j >> 1) & 1);
+                ok = wait(full + 8 * slot, phase) && wait(p_full + 8 * (t & 1), (t >> 1) & 1);
                 tc_fence_after();
                 if (!ok) break;
-                const uint32_t v = slot(v_at(j));
+                const uint64_t v = v_at + slot * (kBlockBytes / 16);
+                const uint32_t probabilities = scores_at + (t & 1) * kKeys;
+                if (elect_one()) {
+                    tc_mma_f16_ts(out_at, probabilities, v, o_desc, j > 0);
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    tc_mma_f16_ts(tm + kOut, tm + (j & 1) * kKeys + k * 8, mnmajor_desc(v + k * 16 * 128, kSpanBytes), o_desc, j > 0 || k > 0);
-                tc_commit(&sm.o_done[j & 1]);
-                release(v_at(j));
+                    for (int k = 1; k < kKeys / 16; ++k) tc_mma_f16_ts(out_at, probabilities + k * 8, v + k * 16 * 128 / 16, o_desc, true);
+                    commit_at(o_done + 8 * (t & 1));
+                    commit_at(empty + 8 * slot);
+                }
+                taken();
             }
-            if (!ok) {      // a wait gave up: the row threads do not wait for what was issued, and the tensor memory is about to be freed
-                tc_commit(&sm.drained);
-                mbar_wait(&sm.drained, 0);
-            }
+        }
+        if (!ok) {      // a wait gave up: the row threads do not wait for what was issued, and the tensor memory is about to be freed
+            if (elect_one()) tc_commit(&sm.drained);
+            mbar_wait(&sm.drained, 0);
         }
     } else {                           // a row's thread
-        const int tok = tok0 + tid / p.group, head = u.kvh * p.group + tid % p.group;
-        const bool valid = tid < p.tile_tokens * p.group && tok < u.n;
-        const bool busy = __any_sync(0xffffffffu, valid);
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, o_at = tm + lanes + kOut;
-        float m = kLowest, l = 0.f;
-        for (int j = 0; j < blocks && ok; ++j) {
-            const int block = u.first + j;
-            if (block >= first_masked) {
-                // values that are none, or that a row may not see and that are no finite numbers, become zeros
-                const int i = j + 1 < blocks ? 2 * j + 2 : 2 * blocks - 1;
-                ok = mbar_wait(&sm.full[i % kSlots], (i / kSlots) & 1) && ok;
-                uint4 *v = reinterpret_cast<uint4 *>(sm.ring[i % kSlots]);
-                const int64_t keys = min(static_cast<int64_t>(u.ctx) + u.n, static_cast<int64_t>(p.width) << p.page_shift) - static_cast<int64_t>(block) * kKeys;
-                bool changed = false;
-#pragma unroll
-                for (int c = 0; c < kBlockBytes / 16 / kRows; ++c) {
-                    const int at = c * kRows + tid, key = (at & (kSpanBytes / 16 - 1)) / 8;
-                    if (key >= keys) {
-                        v[at] = make_uint4(0, 0, 0, 0);
-                        changed = true;
-                        continue;
-                    }
-                    uint4 x = v[at];
-                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    constexpr uint32_t e = Half<T>::kExponent;
-                    if (any_not_finite(w[0], e) || any_not_finite(w[1], e) || any_not_finite(w[2], e) || any_not_finite(w[3], e)) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if ((w[k] & e & 0xffffu) == (e & 0xffffu)) w[k] &= 0xffff0000u;
-                            if ((w[k] & e & 0xffff0000u) == (e & 0xffff0000u)) w[k] &= 0xffffu;
-                        }
-                        v[at] = make_uint4(w[0], w[1], w[2], w[3]);
-                        const int bit = (block - first_masked) * kKeys + key;
-                        if (bit < kMaskedBlocks * 64) atomicOr(&sm.poison[bit >> 5], 1u << (bit & 31));
-                        changed = true;
-                    }
-                }
-                if (changed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
-            ok = mbar_wait(&sm.s_full[j & 1], (j >> 1) & 1) && ok;      // idle warps too: nobody arrives twice in a phase
-            __syncwarp();
-            if (busy) {
-                tc_fence_after();
-                const uint32_t s_at = tm + lanes + (j & 1) * kKeys;
-                uint32_t s[2][32];
-                tmem_ld32(s[0], s_at);
-                tmem_ld32(s[1], s_at + 32);
-                tmem_wait_ld();
-                bool some = true;
+        const f32x2 scale2 = f2_splat(p.scale_log2);
+        const int row_tok = tid / p.group, row_head = tid - row_tok * p.group;
+        int t = 0, fill = 0;
+        for (int segment = 0; ok; ++segment) {
+            ok = wait_at(q_full + 8 * (segment & 1), (segment >> 1) & 1);
+            if (!ok) break;
+            const Segment u = sm.queue[segment % kQueue];
+            if (u.blocks == 0) break;
+            const int tok = u.tok0 + row_tok;
+            const bool valid = tid < p.tile_tokens * p.group && tok < u.n;
+            const bool busy = __any_sync(0xffffffffu, valid);
+            // blocks from here on hold keys that some row does not see, or none
+            const int64_t limit = p.masks ? u.ctx : static_cast<int64_t>(u.ctx) + u.tok0 + 1;
+            const int first_masked = max(u.first, static_cast<int>(limit / kKeys));
+            uint32_t *poison = sm.poison[segment % 3];
+            if (tid < kMaskedBlocks * 2) sm.poison[(segment + 1) % 3][tid] = 0;      // read last before the barrier of the segment in front
+            float m = kLowest, l = 0.f;
+            for (int j = 0; j < u.blocks && ok; ++j, ++t) {
+                const int block = u.first + j;
                 if (block >= first_masked) {
-                    const uint64_t seen = valid ? seen_of(p, u, tok, block * kKeys) : ~0ull;
-                    some = seen != 0;
+                    // values that are none, or that a row may not see and that are no finite numbers, become zeros
+                    const int i = fill + (j + 1 < u.blocks ? 2 * j + 2 : 2 * j + 1);
+                    ok = wait_at(full + 8 * (i % kSlots), (i / kSlots) & 1) && ok;
+                    uint4 *v = reinterpret_cast<uint4 *>(sm.ring[i % kSlots]);
+                    const int keys = static_cast<int>(min(min(static_cast<int64_t>(u.ctx) + u.n, room_of(p)) - static_cast<int64_t>(block) * kKeys, static_cast<int64_t>(kKeys)));
+                    constexpr uint32_t e = Half<T>::kExponent;
+                    constexpr int kMine = kBlockBytes / 16 / kRows;
+                    uint4 x[kMine];
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        if (!(seen >> i & 1)) s[i / 32][i % 32] = 0xff800000u;
-                }
-                float mx[4];
+                    for (int c = 0; c < kMine; ++c) x[c] = v[c * kRows + tid];
+                    uint32_t odd = keys < kKeys;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    mx[c] = __uint_as_float(s[c / 2][(c & 1) * 16]);
+                    for (int c = 0; c < kMine; ++c) odd |= not_finite(x[c].x, e) | not_finite(x[c].y, e) | not_finite(x[c].z, e) | not_finite(x[c].w, e);
+                    const bool changed = odd != 0;
+                    if (changed) {
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c / 2][(c & 1) * 16 + i]));
-                }
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                if (some) top = fmaxf(top, kSeen);
-                const bool grown = top > m + Half<T>::kLag;
-                if (j == 0) {
-                    m = fmaxf(top, kLowest);
-                } else if (__any_sync(0xffffffffu, grown)) {
-                    ok = mbar_wait(&sm.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1) && ok;
-                    __syncwarp();
-                    tc_fence_after();
-                    const float f = grown ? exp2_fast(m - top) : 1.f;
-                    if (grown) m = top, l *= f;
+                        for (int c = 0; c < kMine; ++c) {
+                            const int at = c * kRows + tid, key = (at & (kSpanBytes / 16 - 1)) / 8;
+                            uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+                            if (key >= keys) {
+                                v[at] = make_uint4(0, 0, 0, 0);
+                            } else if (not_finite(w[0], e) | not_finite(w[1], e) | not_finite(w[2], e) | not_finite(w[3], e)) {
 #pragma unroll
-                    for (int c = 0; c < HD; c += 16) {
-                        float o[16];
-                        tmem_ld16(o, o_at + c);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] *= f;
-                        tmem_st16(o_at + c, o);
-                    }
-                }
-                const float shift = Half<T>::kBias - m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t pk[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float a = exp2_fast(fmaf(__uint_as_float(s[i / 16][2 * (i % 16)]), p.scale_log2, shift));
-                    const float c = exp2_fast(fmaf(__uint_as_float(s[i / 16][2 * (i % 16) + 1]), p.scale_log2, shift));
-                    sum[i & 1] += a, sum[2 + (i & 1)] += c;
-                    pk[i] = Half<T>::pack(a, c);
-                }
-                tmem_st32(s_at, pk);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                tc_fence_before();
-            }
-            mbar_arrive(&sm.p_full[j & 1]);
-        }
-        if (blocks > 0 && ok) {
-            ok = mbar_wait(&sm.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1) && ok;
-            tc_fence_after();
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (busy) {
-            uint32_t poison = 0;
-            for (int i = 0; i < kMaskedBlocks * 2; ++i) poison |= sm.poison[i];
-            const bool whole = u.parts == 1;
-            // a row that saw no key is zeros; one whose scores are all -infinity is NaN, as a softmax has it
-            const float r = l == 0.f ? (m > kLowest ? __int_as_float(0x7fffffff) : 0.f) : 1.f / l;
-            T *out = static_cast<T *>(p.out) + static_cast<int64_t>(u.start + tok) * p.out_token + head * p.out_head;
-            float *part = p.partial + (static_cast<int64_t>(u.slot) * kRows + tid) * HD;
-            if (valid && !whole) {
-                float *stats = p.partial + static_cast<int64_t>(p.max_slots) * kRows * HD + static_cast<int64_t>(u.slot) * 2 * kRows + tid;
-                stats[0] = m, stats[kRows] = l;
-            }
-#pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                __syncwarp();
-                if (blocks > 0) {
-                    tmem_ld32(o, o_at + c * 32);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0;
-                }
-                if (poison && valid) {
-                    for (int b = 0; b < kMaskedBlocks * 2; ++b)
-                        for (uint32_t bits = sm.poison[b]; bits; bits &= bits - 1) {
-                            const int bit = b * 32 + __ffs(bits) - 1, block = first_masked + bit / kKeys, key = block * kKeys + bit % kKeys;
-                            if (!(seen_of(p, u, tok, block * kKeys) >> (bit % kKeys) & 1)) continue;
-                            const int64_t page = p.tables[u.request * p.table_stride + (key >> p.page_shift)];
-                            const T *v = static_cast<const T *>(p.v) + page * p.page_stride + u.kvh * p.head_stride + (key & ((1 << p.page_shift) - 1)) * p.row_stride + c * 32;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float x = static_cast<float>(v[i]);
-                                if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+                                for (int k = 0; k < 4; ++k) {
+                                    if ((w[k] & e & 0xffffu) == (e & 0xffffu)) w[k] &= 0xffff0000u;
+                                    if ((w[k] & e & 0xffff0000u) == (e & 0xffff0000u)) w[k] &= 0xffffu;
+                                }
+                                v[at] = make_uint4(w[0], w[1], w[2], w[3]);
+                                const int bit = (block - first_masked) * kKeys + key;
+                                if (bit < kMaskedBlocks * 64) atomicOr(&poison[bit >> 5], 1u << (bit & 31));
                             }
                         }
-                }
-                if (valid && whole) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = Half<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * r, __uint_as_float(o[8 * i + 2 * e + 1]) * r);
-                        reinterpret_cast<uint4 *>(out)[c * 4 + i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                } else if (valid) {
+                    if (changed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                ok = wait_at(s_full + 8 * (t & 1), (t >> 1) & 1) && ok;      // idle warps too: nobody arrives twice in a phase
+                __syncwarp();
+                if (busy) {
+                    tc_fence_after();
+                    const uint32_t s_at = tm + lanes + (t & 1) * kKeys;
+                    uint32_t s[2][32];
+                    tmem_ld32(s[0], s_at);
+                    tmem_ld32(s[1], s_at + 32);
+                    tmem_wait_ld();
+                    bool some = true;
+                    if (block >= first_masked) {
+                        const uint64_t seen = valid ? seen_of(p, u, tok, block * kKeys) : ~0ull;
+                        some = seen != 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) reinterpret_cast<uint4 *>(part)[c * 8 + i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int i = 0; i < 64; ++i)
+                            if (!(seen >> i & 1)) s[i / 32][i % 32] = 0xff800000u;
+                    }
+                    auto score = [&](int i) { return __uint_as_float(s[i / 32][i % 32]); };
+                    float mx[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        mx[c] = fmaxf(score(16 * c), score(16 * c + 1));
+#pragma unroll
+                        for (int i = 2; i < 16; i += 2) mx[c] = max3(mx[c], score(16 * c + i), score(16 * c + i + 1));
+                    }
+                    float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
+                    if (some) top = fmaxf(top, kSeen);
+                    const bool grown = top > m + Half<T>::kLag;
+                    if (j == 0) {
+                        m = fmaxf(top, kLowest);
+                    } else if (__any_sync(0xffffffffu, grown)) {
+                        ok = wait_at(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1) && ok;
+                        __syncwarp();
+                        tc_fence_after();
+                        const float f = grown ? exp2_fast(m - top) : 1.f;
+                        if (grown) m = top, l *= f;
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 16) {
+                            float o[16];
+                            tmem_ld16(o, o_at + c);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] *= f;
+                            tmem_st16(o_at + c, o);
+                        }
+                    }
+                    const f32x2 shift2 = f2_splat(Half<T>::kBias - m);
+                    f32x2 sum[2] = {0, 0};
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float a, c;
+                        f2_split(f2_fma(f2_make_bits(s[i / 16][2 * (i % 16)], s[i / 16][2 * (i % 16) + 1]), scale2, shift2), a, c);
+                        a = exp2_fast(a), c = exp2_fast(c);
+                        sum[i & 1] = f2_add(sum[i & 1], f2_make(a, c));
+                        pk[i] = Half<T>::pack(a, c);
+                    }
+                    tmem_st32(s_at, pk);
+                    l += f2_sum(f2_add(sum[0], sum[1]));
+                    tmem_wait_st();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if ((tid & 31) == 0) arrive_at(p_full + 8 * (t & 1));
+            }
+            fill += 2 * u.blocks;
+            if (ok) ok = wait_at(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
+            tc_fence_after();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (busy) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int i = 0; i < kMaskedBlocks * 2; ++i) any |= poison[i];
+                const bool whole = u.slot < 0;
+                // a row that saw no key is zeros; one whose scores are all -infinity is NaN, as a softmax has it
+                const float r = l == 0.f ? (m > kLowest ? __int_as_float(0x7fffffff) : 0.f) : 1.f / l;
+                const int head = u.kvh * p.group + row_head;
+                T *out = static_cast<T *>(p.out) + static_cast<int64_t>(u.start + tok) * p.out_token + head * p.out_head;
+                uint4 *part = reinterpret_cast<uint4 *>(p.partial) + static_cast<int64_t>(u.slot) * (HD / 4) * kRows + tid;
+                if (valid && !whole) {
+                    float *stats = p.stats + static_cast<int64_t>(u.slot) * 2 * kRows + tid;
+                    stats[0] = m, stats[kRows] = l;
+                }
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tmem_ld32(o, o_at + c * 32);
+                    tmem_wait_ld();
+                    if (any && valid) {
+                        for (int b = 0; b < kMaskedBlocks * 2; ++b)
+                            for (uint32_t bits = poison[b]; bits; bits &= bits - 1) {
+                                const int bit = b * 32 + __ffs(bits) - 1, block = first_masked + bit / kKeys, key = block * kKeys + bit % kKeys;
+                                if (!(seen_of(p, u, tok, block * kKeys) >> (bit % kKeys) & 1)) continue;
+                                const int64_t page = p.tables[u.request * p.table_stride + (key >> p.page_shift)];
+                                const T *v = static_cast<const T *>(p.v) + page * p.page_stride + u.kvh * p.head_stride + (key & ((1 << p.page_shift) - 1)) * p.row_stride + c * 32;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float x = static_cast<float>(v[i]);
+                                    if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+                                }
+                            }
+                    }
+                    if (valid && whole) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) w[e] = Half<T>::pack(__uint_as_float(o[16 * i + 2 * e]) * r, __uint_as_float(o[16 * i + 2 * e + 1]) * r);
+                            if (p.out_sectors) {
+                                store_sector(out + c * 32 + i * 16, w);
+                            } else {
+                                reinterpret_cast<uint4 *>(out)[c * 4 + 2 * i] = make_uint4(w[0], w[1], w[2], w[3]);
+                                reinterpret_cast<uint4 *>(out)[c * 4 + 2 * i + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+                            }
+                        }
+                    } else if (valid) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) part[(c * 8 + i) * kRows] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
                 }
             }
         }
+        // the product before the last has been counted too before the CTA ends
+        if (ok && t > 1) ok = wait_at(o_done + 8 * (t & 1), ((t - 2) >> 1) & 1);
     }
     if (!ok) *p.status = 1;
     tc_fence_before();
@@ -533,38 +671,68 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     }
 }
 
-// Parts of a tile joined, a warp per row: weights from the parts' maxima, sums in the order of the parts.
-constexpr int kJoinThreads = 256;
+// Parts of a tile joined: the one that the CTA where the tile begins left, and those of the CTAs behind it up to the tile's last, in that order.  A CTA takes 32 rows of a tile, a lane
+// for each; its eight warps read the statistics of as many parts at a time, and then each an eighth of the values of all parts.
+constexpr int kJoinWarps = 8, kJoinCtas = kRows / 32, kJoinParts = 32;
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ PagedAttentionParams p) {
-    constexpr int kVec = HD / 32;      // values a lane
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PagedAttentionParams p) {
+    constexpr int kVecs = HD / 4 / kJoinWarps, kAhead = 16 / kVecs;      // vectors of four that a lane sums up, and parts of them that it reads at a time
+    __shared__ float maxima[kJoinParts][32], sums[kJoinParts][32];
+    __shared__ int slots[kJoinParts];
     grid_dependency_sync();
-    const int lane = threadIdx.x & 31;
-    const int64_t rows = static_cast<int64_t>(p.units[0]) * kRows;
-    for (int64_t at = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); at < rows; at += static_cast<int64_t>(gridDim.x) * (kJoinThreads / 32)) {
-        const Unit u = reinterpret_cast<const Unit *>(p.units + 4)[at / kRows];
-        const int row = static_cast<int>(at % kRows), tok = u.tile * p.tile_tokens + row / p.group;
-        if (row >= p.tile_tokens * p.group || tok >= u.n) continue;
-        const float *stats = p.partial + static_cast<int64_t>(p.max_slots) * kRows * HD + static_cast<int64_t>(u.slot) * 2 * kRows + row;
-        const float *part = p.partial + (static_cast<int64_t>(u.slot) * kRows + row) * HD + lane * kVec;
-        float top = kLowest;
-        for (int s = lane; s < u.parts; s += 32) top = fmaxf(top, stats[s * 2 * kRows]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float acc[kVec] = {}, total = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < u.parts; ++s) {
-            const float w = exp2f(stats[s * 2 * kRows] - top);
-            total += w * stats[s * 2 * kRows + kRows];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) acc[i] += w * part[static_cast<int64_t>(s) * kRows * HD + i];
+    const int cta = blockIdx.x / kJoinCtas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = p.joints[0].ctas;
+    if (cta >= ctas) return;
+    const Segment u = p.joints[cta].open;
+    const int row = blockIdx.x % kJoinCtas * 32 + lane, tok = u.tok0 + row / p.group;
+    const bool valid = u.slot >= 0 && row < p.tile_tokens * p.group && tok < u.n;
+    if (!__any_sync(0xffffffffu, valid)) return;      // the same in all warps
+    const float4 *partial = reinterpret_cast<const float4 *>(p.partial) + warp * kVecs * kRows + row;
+    float top = kLowest, total = 0.f;
+    float4 acc[kVecs] = {};
+    for (int next = cta; next < ctas; next += 32) {      // 32 CTAs at a time, a lane for each
+        const int c = next + lane;
+        const int head = c >= ctas ? 0 : c == cta ? 1 : p.joints[c].head;
+        const uint32_t over = __ballot_sync(0xffffffffu, c >= ctas || head >= 2);
+        const int reach = over ? __ffs(over) : 32;
+        const bool mine = lane < reach && (head == 1 || head == 2);
+        const uint32_t parts = __ballot_sync(0xffffffffu, mine);
+        const int count = __popc(parts);
+        __syncthreads();      // the last 32 have been read
+        if (warp == 0 && mine) slots[__popc(parts & ((1u << lane) - 1))] = c == cta ? u.slot : 2 * c;
+        __syncthreads();
+        for (int i = warp; i < count; i += kJoinWarps) {
+            const float *stats = p.stats + static_cast<int64_t>(slots[i]) * 2 * kRows + row;
+            maxima[i][lane] = stats[0], sums[i][lane] = stats[kRows];
         }
-        const float r = total == 0.f ? (top > kLowest ? __int_as_float(0x7fffffff) : 0.f) : 1.f / total;
-        uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) + static_cast<int64_t>(u.start + tok) * p.out_token +
-                                                     (u.kvh * p.group + row % p.group) * p.out_head + lane * kVec);
+        __syncthreads();
+        float high = top;
+        for (int i = 0; i < count; ++i) high = fmaxf(high, maxima[i][lane]);
+        const float fade = exp2f(top - high);
+        top = high, total *= fade;
 #pragma unroll
-        for (int i = 0; i < kVec / 2; ++i) out[i] = Half<T>::pack(acc[2 * i] * r, acc[2 * i + 1] * r);
+        for (int k = 0; k < kVecs; ++k) acc[k].x *= fade, acc[k].y *= fade, acc[k].z *= fade, acc[k].w *= fade;
+        for (int i = 0; i < count; i += kAhead) {
+            float4 v[kAhead][kVecs];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                for (int k = 0; k < kVecs; ++k) v[a][k] = partial[(static_cast<int64_t>(slots[min(i + a, count - 1)]) * (HD / 4) + k) * kRows];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (i + a < count) {
+                    const float w = exp2f(maxima[i + a][lane] - top);
+                    total += w * sums[i + a][lane];
+#pragma unroll
+                    for (int k = 0; k < kVecs; ++k) acc[k].x += w * v[a][k].x, acc[k].y += w * v[a][k].y, acc[k].z += w * v[a][k].z, acc[k].w += w * v[a][k].w;
+                }
+        }
+        if (over) break;
     }
+    if (!valid) return;
+    const float r = total == 0.f ? (top > kLowest ? __int_as_float(0x7fffffff) : 0.f) : 1.f / total;
+    uint2 *out = reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + static_cast<int64_t>(u.start + tok) * p.out_token + (u.kvh * p.group + row % p.group) * p.out_head) + warp * kVecs;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) out[k] = make_uint2(Half<T>::pack(acc[k].x * r, acc[k].y * r), Half<T>::pack(acc[k].z * r, acc[k].w * r));
 }
 
 struct Kernels {
@@ -582,23 +750,20 @@ Kernels kernels_of(int dtype, int head_dim) {
 
 // What a call is cut into at most.
 struct Shape {
-    int group, tile_tokens, target, may_split;
-    int64_t tiles;      // times kv heads
-    int64_t grid, slots, bytes;
+    int group, tile_tokens, may_split;
+    int64_t grid, bytes;
 };
 Shape shape_of(int batch, int tokens, int heads, int kv_heads, int head_dim, int64_t max_len, int sms) {
     Shape s = {};
     s.group = heads / kv_heads;
     s.tile_tokens = kRows / s.group;
-    s.target = sms * kCtasPerSm;
     // sum of ceil(n / t) <= floor(sum of n / t) + requests with new tokens
     const int64_t full = tokens / s.tile_tokens, some = batch < tokens ? batch : tokens;
-    s.tiles = (full + some < tokens ? full + some : tokens) * kv_heads;
-    s.may_split = max_len > kMinPart * kKeys;
-    // a part has at least work / target blocks: all parts are at most tiles + target, those of tiles in parts at most 2 * target
-    s.grid = s.tiles + (s.may_split ? s.target : 0);
-    s.slots = s.may_split ? 2 * s.target : 0;
-    s.bytes = s.may_split ? 16 + s.target * static_cast<int64_t>(sizeof(Unit)) + s.slots * kRows * (head_dim + 2) * 4 : 0;
+    const int64_t tiles = (full + some < tokens ? full + some : tokens) * kv_heads;
+    s.may_split = max_len + kTileCost >= 2 * kGrain;      // shorter tiles are never cut
+    const int64_t most = static_cast<int64_t>(sms) * kCtasPerSm, want = 2 * tiles + tiles * (max_len + kTileCost) / kPerCta;
+    s.grid = tiles >= most || want >= most ? most : want;
+    s.bytes = s.may_split ? s.grid * (static_cast<int64_t>(sizeof(Joint)) + 2ll * kRows * (head_dim + 2) * 4) : 0;
     return s;
 }
 
@@ -655,6 +820,7 @@ extern "C" int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64
     if (p2 < 8 || (p2 & (p2 - 1)) || p2 > 65536) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: pages of %d tokens; built for powers of two from 8 to 65536", p2);
     if (masks && mask_words > 8) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: masks of %d words; built for at most 8 (256 new tokens of a request)", mask_words);
     if (static_cast<int64_t>(table_width) * p2 > 0x7fffff00ll) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: a table of %d pages is too wide", table_width);
+    if (tokens > 1 << 24) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: %d new tokens; built for at most 2^24", tokens);
     if (batch == 0 || tokens == 0) return GPUK_OK;
     if (!q || !lens || !starts || !out || (table_width > 0 && !tables)) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
     if (pages->num_pages == 0 || table_width == 0 || !pages->k || !pages->v) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: no pages");
@@ -666,7 +832,6 @@ extern "C" int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64
     rc = decode_device(&d);
     if (rc != GPUK_OK) return rc;
     Shape s = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms);
-    if (s.grid > 0x7fffffffll) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: too many tokens");
     if (s.may_split && (!workspace || workspace_bytes < s.bytes || !aligned16(workspace)))
         return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: needs a workspace of %lld bytes, 16-byte aligned", static_cast<long long>(s.bytes));
     const int hd = pages->head_dim;
@@ -684,17 +849,18 @@ extern "C" int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64
     if (e) return set_last_error(GPUK_ERR_CUDA, "paged_attention: the driver refused a tensor map (%d)", e);
     int shift = 0;
     while ((1 << shift) < p2) ++shift;
-    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    Joint *joints = static_cast<Joint *>(workspace);
+    float *partial = reinterpret_cast<float *>(joints + s.grid);
     PagedAttentionParams p = {tables, lens, starts, masks, pages->v, out, table_stride, pages->page_stride, pages->head_stride, pages->row_stride, pages->num_pages,
-                              out_token_stride, out_head_stride, batch, tokens, pages->kv_heads, s.group, s.tile_tokens, mask_words, table_width, shift, s.target, s.may_split,
-                              scale * 1.4426950408889634f, d->status, reinterpret_cast<int *>(ws), reinterpret_cast<float *>(ws + 16 + s.target * sizeof(Unit)),
-                              static_cast<int>(s.slots)};
+                              out_token_stride, out_head_stride, batch, tokens, pages->kv_heads, s.group, s.tile_tokens, mask_words, static_cast<uint32_t>(((1ull << 32) + s.tile_tokens - 1) / s.tile_tokens), table_width, shift, s.may_split,
+                              (reinterpret_cast<uintptr_t>(out) | out_token_stride * 2 | out_head_stride * 2) % 32 == 0,
+                              scale * 1.4426950408889634f, d->status, joints, partial, partial + s.grid * 2 * kRows * hd};
     const Kernels k = kernels_of(pages->dtype, hd);
     void *args[] = {&qmap, &kmap, &vmap, &p};
     cudaError_t err = launch_kernel(k.attend, static_cast<int>(s.grid), kThreads, 1, false, args, static_cast<cudaStream_t>(stream), k.smem);
     if (err == cudaSuccess && s.may_split) {
         void *join_args[] = {&p};
-        err = launch_kernel(k.join, 4 * d->sms, kJoinThreads, 1, false, join_args, static_cast<cudaStream_t>(stream));
+        err = launch_kernel(k.join, static_cast<int>(s.grid) * kJoinCtas, kJoinWarps * 32, 1, false, join_args, static_cast<cudaStream_t>(stream));
     }
     if (err != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_attention: launch failed: %s", cudaGetErrorString(err));
     return GPUK_OK;
