@@ -43,7 +43,8 @@ constexpr int kOut = 2 * kKeys;                  // first column of the outputs
 constexpr int kMaskedBlocks = 8;                 // that a tile can have
 constexpr int kCtasPerSm = 2;
 constexpr int kTileCost = 4 * kKeys;             // what a tile costs beside its keys, in keys: its queries, its outputs, the first scores
-constexpr int kGrain = kTileCost + 2 * kKeys;    // no tile is cut nearer than that to one of its ends
+constexpr int kGrain = 2 * kKeys;                // no tile is cut nearer than that to its end, or than kFront to its beginning
+constexpr int kFront = 3 * kKeys;
 constexpr int kPerCta = 256;                     // keys for which a call takes another CTA
 constexpr int kQueue = 4;                        // segments that are described at a time
 
@@ -191,7 +192,8 @@ __device__ __forceinline__ int64_t keys_of(const PagedAttentionParams &p, const 
     const int64_t most = static_cast<int64_t>(r.ctx) + (p.masks ? static_cast<int64_t>(r.n) : min(static_cast<int64_t>(r.n), static_cast<int64_t>(tile + 1) * p.tile_tokens));
     return min(most, room_of(p));
 }
-// The weight of the tiles in front of one.
+// The weight of a tile, and of those in front of one.
+__device__ __forceinline__ int64_t weight_of(const PagedAttentionParams &p, const Request &r, int tile) { return kTileCost + (r.over ? room_of(p) : keys_of(p, r, tile)); }
 __device__ __forceinline__ int64_t weight_before(const PagedAttentionParams &p, const Request &r, int tile) {
     if (r.tiles == 0) return 0;
     if (p.masks || r.over) return tile * (kTileCost + min(static_cast<int64_t>(r.ctx) + r.n, room_of(p)));
@@ -222,7 +224,8 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
     const int few = __reduce_add_sync(0xffffffffu, static_cast<int>(min(tiles, static_cast<int64_t>(1 << 20))));
     const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), 2 * few + all / kPerCta));
     const int border = static_cast<int>(blockIdx.x) + side;
-    const int64_t raw = border < ctas ? static_cast<int64_t>(static_cast<double>(all) / ctas * border) : all;
+    const int64_t share = static_cast<int64_t>(static_cast<float>(all) * (1.00001f / ctas)) + 1;      // the last CTA's is a little shorter
+    const int64_t raw = min(all, border * share);
     if (raw >= all) {      // the line's end
         if (lane == 0) out->x[side] = all, out->ctas = ctas;
         return;
@@ -236,19 +239,21 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
             base += here;
             continue;
         }
-        int64_t at = raw - base;
-        int kvh = min(p.kv_heads - 1, static_cast<int>(__fdividef(static_cast<float>(at), static_cast<float>(head))));
+        int64_t at = raw - base, first = 0;
+        int kvh = min(p.kv_heads - 1, static_cast<int>(__fdividef(static_cast<float>(at), static_cast<float>(head)))), tile = 0;
         while (kvh > 0 && kvh * head > at) --kvh;
         while (kvh + 1 < p.kv_heads && (kvh + 1) * head <= at) ++kvh;
         at -= kvh * head;
-        // weight_before(tile) <= at < weight_before(tile + 1): a line, or a parabola with half a tile's tokens to the square
-        const float slope = kTileCost + r.ctx + (p.masks || r.over ? static_cast<float>(r.n) : 0.5f * p.tile_tokens), bend = p.masks || r.over ? 0.f : 0.5f * p.tile_tokens;
-        int tile = min(r.tiles - 1, static_cast<int>(bend == 0.f ? static_cast<float>(at) / slope : (sqrtf(slope * slope + 4.f * bend * at) - slope) / (2.f * bend)));
-        while (tile > 0 && weight_before(p, r, tile) > at) --tile;
-        while (tile + 1 < r.tiles && weight_before(p, r, tile + 1) <= at) ++tile;
-        const int64_t first = weight_before(p, r, tile), size = weight_before(p, r, tile + 1) - first;
+        if (r.tiles > 1) {      // weight_before(tile) <= at < weight_before(tile + 1): a line, or a parabola with half a tile's tokens to the square
+            const float slope = kTileCost + r.ctx + (p.masks || r.over ? static_cast<float>(r.n) : 0.5f * p.tile_tokens), bend = p.masks || r.over ? 0.f : 0.5f * p.tile_tokens;
+            tile = min(r.tiles - 1, static_cast<int>(bend == 0.f ? static_cast<float>(at) / slope : (sqrtf(slope * slope + 4.f * bend * at) - slope) / (2.f * bend)));
+            while (tile > 0 && weight_before(p, r, tile) > at) --tile;
+            while (tile + 1 < r.tiles && weight_before(p, r, tile + 1) <= at) ++tile;
+            first = weight_before(p, r, tile);
+        }
+        const int64_t size = weight_of(p, r, tile);
         int64_t pos = at - first;
-        if (!p.may_split || r.over || pos < kGrain) pos = 0;
+        if (!p.may_split || r.over || pos < kTileCost + kFront) pos = 0;
         else if (size - pos < kGrain) pos = size;
         else pos = pos / kKeys * kKeys;      // the borders of blocks, behind the tile's cost
         out->x[side] = base + kvh * head + first + pos, out->ctas = ctas;
@@ -265,7 +270,7 @@ struct Walk {
     __device__ explicit Walk(const Start &s) : r(s.r), request(s.request), kvh(s.kvh), tile(s.tile), index(0), pos(s.pos), left(s.x[1] - s.x[0]) {}
     __device__ bool next(const PagedAttentionParams &p, Segment *out, bool *begins, bool *ends) {
         if (left <= 0) return false;
-        int64_t size = weight_before(p, r, tile + 1) - weight_before(p, r, tile);
+        int64_t size = weight_of(p, r, tile);
         while (pos >= size) {      // at a tile's end, to the next
             pos = 0;
             if (++tile >= r.tiles) {
@@ -278,7 +283,7 @@ struct Walk {
                     } while (r.tiles == 0);
                 }
             }
-            size = weight_before(p, r, tile + 1) - weight_before(p, r, tile);
+            size = weight_of(p, r, tile);
         }
         const int64_t take = min(size - pos, left), end = pos + take;
         const int all = static_cast<int>((keys_of(p, r, tile) + kKeys - 1) / kKeys);
@@ -320,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     if (tid == kRows + 32) prefetch_map(&qmap), prefetch_map(&kmap), prefetch_map(&vmap);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp < 2) find_border(p, &sm.start, warp);
+    if (warp == kRows / 32) tmem_alloc<kColumns>(&sm.tmem);
     if (tid == kRows) {
         for (int b = 0; b < 2; ++b) mbar_init(&sm.q_full[b], 1), mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows / 32), mbar_init(&sm.o_done[b], 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
@@ -328,14 +334,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     }
     if (tid >= kRows + 32)
         for (int i = tid - kRows - 32; i < 3 * kMaskedBlocks * 2; i += 32) sm.poison[0][i] = 0;
+    tc_fence_before();
     __syncthreads();
     if (sm.start.x[1] <= sm.start.x[0]) {      // a border that went to an end of its tile, or fewer CTAs than there are
         if (tid == 0 && p.may_split) p.joints[blockIdx.x].open.slot = -1, p.joints[blockIdx.x].head = 0, p.joints[blockIdx.x].ctas = sm.start.ctas;
+        if (warp == kRows / 32) tmem_free<kColumns>(sm.tmem);
         return;
     }
-    if (warp == kRows / 32) tmem_alloc<kColumns>(&sm.tmem);
-    tc_fence_before();
-    __syncthreads();
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // behind the allocation: no CTA that follows takes columns one of this grid waits for
     const uint32_t tm = sm.tmem;
@@ -391,17 +396,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                 from += boxes, --left;
                 return page;
             };
+            auto load_q = [&]() {
+                if (lane == 0) {
+                    sm.queue[segments % kQueue] = u;
+                    expect_at(q_full + 8 * (segments & 1), kSpans * p.tile_tokens * p.group * 128);
+#pragma unroll
+                    for (int h = 0; h < kSpans; ++h) tma_load_3d(smem_addr(sm.q) + h * kQSpanBytes, &qmap, h * 64, u.kvh * p.group, u.start + u.tok0, &sm.q_full[segments & 1]);
+                }
+            };
+            if (segments == 0) load_q();      // the first keys wait for the table, those of later segments for nothing
             int page_k = next_page(0);
             ok = load(&kmap, 0, page_k);
-            if (ok && segments > 0) ok = wait_at(q_empty, (segments - 1) & 1);
-            if (!ok) break;
-            if (lane == 0) {
-                const uint32_t bar = q_full + 8 * (segments & 1);
-                sm.queue[segments % kQueue] = u;
-                expect_at(bar, kSpans * p.tile_tokens * p.group * 128);
-#pragma unroll
-                for (int h = 0; h < kSpans; ++h) tma_load_3d(smem_addr(sm.q) + h * kQSpanBytes, &qmap, h * 64, u.kvh * p.group, u.start + u.tok0, &sm.q_full[segments & 1]);
+            if (ok && segments > 0) {
+                ok = wait_at(q_empty, (segments - 1) & 1);
+                if (ok) load_q();
             }
+            if (!ok && segments > 0) break;
             ++segments;
             for (int j = 0; ok && j < u.blocks; ++j) {
                 const int page_v = page_k;
@@ -500,42 +510,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             float m = kLowest, l = 0.f;
             for (int j = 0; j < u.blocks && ok; ++j, ++t) {
                 const int block = u.first + j;
-                if (block >= first_masked) {
-                    // values that are none, or that a row may not see and that are no finite numbers, become zeros
-                    const int i = fill + (j + 1 < u.blocks ? 2 * j + 2 : 2 * j + 1);
-                    ok = wait_at(full + 8 * (i % kSlots), (i / kSlots) & 1) && ok;
-                    uint4 *v = reinterpret_cast<uint4 *>(sm.ring[i % kSlots]);
-                    const int keys = static_cast<int>(min(min(static_cast<int64_t>(u.ctx) + u.n, room_of(p)) - static_cast<int64_t>(block) * kKeys, static_cast<int64_t>(kKeys)));
-                    constexpr uint32_t e = Half<T>::kExponent;
-                    constexpr int kMine = kBlockBytes / 16 / kRows;
-                    uint4 x[kMine];
-#pragma unroll
-                    for (int c = 0; c < kMine; ++c) x[c] = v[c * kRows + tid];
-                    uint32_t odd = keys < kKeys;
-#pragma unroll
-                    for (int c = 0; c < kMine; ++c) odd |= not_finite(x[c].x, e) | not_finite(x[c].y, e) | not_finite(x[c].z, e) | not_finite(x[c].w, e);
-                    const bool changed = odd != 0;
-                    if (changed) {
-#pragma unroll
-                        for (int c = 0; c < kMine; ++c) {
-                            const int at = c * kRows + tid, key = (at & (kSpanBytes / 16 - 1)) / 8;
-                            uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-                            if (key >= keys) {
-                                v[at] = make_uint4(0, 0, 0, 0);
-                            } else if (not_finite(w[0], e) | not_finite(w[1], e) | not_finite(w[2], e) | not_finite(w[3], e)) {
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if ((w[k] & e & 0xffffu) == (e & 0xffffu)) w[k] &= 0xffff0000u;
-                                    if ((w[k] & e & 0xffff0000u) == (e & 0xffff0000u)) w[k] &= 0xffffu;
-                                }
-                                v[at] = make_uint4(w[0], w[1], w[2], w[3]);
-                                const int bit = (block - first_masked) * kKeys + key;
-                                if (bit < kMaskedBlocks * 64) atomicOr(&poison[bit >> 5], 1u << (bit & 31));
-                            }
-                        }
-                    }
-                    if (changed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
                 ok = wait_at(s_full + 8 * (t & 1), (t >> 1) & 1) && ok;      // idle warps too: nobody arrives twice in a phase
                 __syncwarp();
                 if (busy) {
@@ -597,6 +571,42 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                     l += f2_sum(f2_add(sum[0], sum[1]));
                     tmem_wait_st();
                     tc_fence_before();
+                }
+                if (block >= first_masked) {
+                    // values that are none, or that a row may not see and that are no finite numbers, become zeros
+                    const int i = fill + (j + 1 < u.blocks ? 2 * j + 2 : 2 * j + 1);
+                    ok = wait_at(full + 8 * (i % kSlots), (i / kSlots) & 1) && ok;
+                    uint4 *v = reinterpret_cast<uint4 *>(sm.ring[i % kSlots]);
+                    const int keys = static_cast<int>(min(min(static_cast<int64_t>(u.ctx) + u.n, room_of(p)) - static_cast<int64_t>(block) * kKeys, static_cast<int64_t>(kKeys)));
+                    constexpr uint32_t e = Half<T>::kExponent;
+                    constexpr int kMine = kBlockBytes / 16 / kRows;
+                    uint4 x[kMine];
+#pragma unroll
+                    for (int c = 0; c < kMine; ++c) x[c] = v[c * kRows + tid];
+                    uint32_t odd = keys < kKeys;
+#pragma unroll
+                    for (int c = 0; c < kMine; ++c) odd |= not_finite(x[c].x, e) | not_finite(x[c].y, e) | not_finite(x[c].z, e) | not_finite(x[c].w, e);
+                    const bool changed = odd != 0;
+                    if (changed) {
+#pragma unroll
+                        for (int c = 0; c < kMine; ++c) {
+                            const int at = c * kRows + tid, key = (at & (kSpanBytes / 16 - 1)) / 8;
+                            uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+                            if (key >= keys) {
+                                v[at] = make_uint4(0, 0, 0, 0);
+                            } else if (not_finite(w[0], e) | not_finite(w[1], e) | not_finite(w[2], e) | not_finite(w[3], e)) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    if ((w[k] & e & 0xffffu) == (e & 0xffffu)) w[k] &= 0xffff0000u;
+                                    if ((w[k] & e & 0xffff0000u) == (e & 0xffff0000u)) w[k] &= 0xffffu;
+                                }
+                                v[at] = make_uint4(w[0], w[1], w[2], w[3]);
+                                const int bit = (block - first_masked) * kKeys + key;
+                                if (bit < kMaskedBlocks * 64) atomicOr(&poison[bit >> 5], 1u << (bit & 31));
+                            }
+                        }
+                    }
+                    if (changed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();
                 if ((tid & 31) == 0) arrive_at(p_full + 8 * (t & 1));
@@ -672,11 +682,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
 }
 
 // Parts of a tile joined: the one that the CTA where the tile begins left, and those of the CTAs behind it up to the tile's last, in that order.  A CTA takes 32 rows of a tile, a lane
-// for each; its eight warps read the statistics of as many parts at a time, and then each an eighth of the values of all parts.
+// for each; its warps read the statistics of as many parts at a time, and then each its share of the values of all parts.
 constexpr int kJoinWarps = 8, kJoinCtas = kRows / 32, kJoinParts = 32;
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PagedAttentionParams p) {
-    constexpr int kVecs = HD / 4 / kJoinWarps, kAhead = 16 / kVecs;      // vectors of four that a lane sums up, and parts of them that it reads at a time
+__global__ void __launch_bounds__(kJoinWarps * 32, 3) join_kernel(const __grid_constant__ PagedAttentionParams p) {
+    constexpr int kVecs = HD / 4 / kJoinWarps, kAhead = 8 / kVecs;      // vectors of four that a lane sums up, and parts of them that it reads at a time
     __shared__ float maxima[kJoinParts][32], sums[kJoinParts][32];
     __shared__ int slots[kJoinParts];
     grid_dependency_sync();
@@ -700,6 +710,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
         __syncthreads();      // the last 32 have been read
         if (warp == 0 && mine) slots[__popc(parts & ((1u << lane) - 1))] = c == cta ? u.slot : 2 * c;
         __syncthreads();
+#pragma unroll 2
         for (int i = warp; i < count; i += kJoinWarps) {
             const float *stats = p.stats + static_cast<int64_t>(slots[i]) * 2 * kRows + row;
             maxima[i][lane] = stats[0], sums[i][lane] = stats[kRows];
@@ -760,7 +771,7 @@ Shape shape_of(int batch, int tokens, int heads, int kv_heads, int head_dim, int
     // sum of ceil(n / t) <= floor(sum of n / t) + requests with new tokens
     const int64_t full = tokens / s.tile_tokens, some = batch < tokens ? batch : tokens;
     const int64_t tiles = (full + some < tokens ? full + some : tokens) * kv_heads;
-    s.may_split = max_len + kTileCost >= 2 * kGrain;      // shorter tiles are never cut
+    s.may_split = max_len >= kFront + kGrain;      // shorter tiles are never cut
     const int64_t most = static_cast<int64_t>(sms) * kCtasPerSm, want = 2 * tiles + tiles * (max_len + kTileCost) / kPerCta;
     s.grid = tiles >= most || want >= most ? most : want;
     s.bytes = s.may_split ? s.grid * (static_cast<int64_t>(sizeof(Joint)) + 2ll * kRows * (head_dim + 2) * 4) : 0;

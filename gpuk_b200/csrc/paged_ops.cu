@@ -31,87 +31,98 @@ struct PlanParams {
     int batch, width, page_shift, capacity, total, words;
 };
 
-// Sums of a, b and c over the threads in front, and over all of them.
-struct Sums {
-    int64_t a, b, c;
+// Sums over the threads in front, and over all of them, that stay at a ceiling once they reach it.
+constexpr int kCeiling = 0x3fffffff;
+struct Saturated {
+    int v;
+    __device__ Saturated operator+(Saturated o) const { return {min(v + o.v, kCeiling)}; }
+    __device__ Saturated up(int lanes) const { return {__shfl_up_sync(0xffffffffu, v, lanes)}; }
+    __device__ Saturated at(int lane) const { return {__shfl_sync(0xffffffffu, v, lane)}; }
 };
-__device__ Sums block_before(Sums v, Sums *all, Sums (&warp_sums)[kPlanWarps]) {
+// Two sums at once, each below 2^31.
+struct Pair {
+    int a, b;
+    __device__ Pair operator+(Pair o) const { return {a + o.a, b + o.b}; }
+    __device__ Pair up(int lanes) const { return {__shfl_up_sync(0xffffffffu, a, lanes), __shfl_up_sync(0xffffffffu, b, lanes)}; }
+    __device__ Pair at(int lane) const { return {__shfl_sync(0xffffffffu, a, lane), __shfl_sync(0xffffffffu, b, lane)}; }
+};
+template <typename V>
+__device__ V warp_upto(V v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V t = v.up(o);
+        if (lane >= o) v = v + t;
+    }
+    return v;
+}
+// `before`: the sum of the threads in front; returns that of all.
+template <typename V>
+__device__ V block_before(V v, V *before, V (&warp_sums)[kPlanWarps + 1]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Sums s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const Sums t = {__shfl_up_sync(0xffffffffu, s.a, o), __shfl_up_sync(0xffffffffu, s.b, o), __shfl_up_sync(0xffffffffu, s.c, o)};
-        if (lane >= o) s.a += t.a, s.b += t.b, s.c += t.c;
-    }
+    const V upto = warp_upto(v), front = upto.up(1);
+    __syncthreads();      // the sums have been read
+    if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
-    if (lane == 31) warp_sums[warp] = s;
-    __syncthreads();
-    Sums w = warp_sums[lane], u = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const Sums t = {__shfl_up_sync(0xffffffffu, u.a, o), __shfl_up_sync(0xffffffffu, u.b, o), __shfl_up_sync(0xffffffffu, u.c, o)};
-        if (lane >= o) u.a += t.a, u.b += t.b, u.c += t.c;
-    }
-    *all = {__shfl_sync(0xffffffffu, u.a, 31), __shfl_sync(0xffffffffu, u.b, 31), __shfl_sync(0xffffffffu, u.c, 31)};
-    const Sums f = {__shfl_sync(0xffffffffu, u.a - w.a, warp), __shfl_sync(0xffffffffu, u.b - w.b, warp), __shfl_sync(0xffffffffu, u.c - w.c, warp)};
-    return {f.a + s.a - v.a, f.b + s.b - v.b, f.c + s.c - v.c};
+    const V sums = warp_upto(warp_sums[lane]), others = sums.at(max(warp - 1, 0)), all = sums.at(31);
+    *before = warp == 0 ? V{} : others;
+    if (lane > 0) *before = *before + front;
+    return all;
 }
 
+// Tokens a thread places at a time, and the parents that its CTA keeps at hand for them: those of the tokens, and of the request that goes on from in front of them.
+constexpr int kTokens = 2, kSpan = kTokens * kPlanThreads, kBehind = 256;
+
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams p) {
-    extern __shared__ int32_t lists[];      // per request: first token, the pages in front that come back or go out, and those that it holds
-    __shared__ Sums warp_sums[kPlanWarps];
-    int32_t *const starts = lists, *const back_at = starts + p.batch + 1, *const want_at = back_at + p.batch, *const holds = want_at + p.batch;
+    extern __shared__ int32_t lists[];      // per request: first token, cached tokens, the pages in front that come back or go out, and those that it holds
+    __shared__ Saturated token_sums[kPlanWarps + 1];
+    __shared__ Pair page_sums[kPlanWarps + 1];
+    __shared__ int32_t family[kSpan + kBehind];
+    __shared__ unsigned long long over;      // pages for which the rows of the table have no room
+    int32_t *const starts = lists, *const lens = starts + p.batch + 1, *const back_at = lens + p.batch, *const want_at = back_at + p.batch, *const holds = want_at + p.batch;
     const int ctas = cluster_size(), cta = cluster_cta_rank(), tid = threadIdx.x, lane = tid & 31;
-    const int64_t thread = static_cast<int64_t>(cta) * kPlanThreads + tid, threads = static_cast<int64_t>(ctas) * kPlanThreads;
+    const int thread = cta * kPlanThreads + tid, threads = ctas * kPlanThreads;
+    if (tid == 0) over = 0;
     grid_dependency_sync();
     const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
     const int page = 1 << p.page_shift;
 
     struct Need {
-        int64_t lens;
         int held, need;
-        int64_t over;
     };
-    auto need_of = [&](int i, int n) {
-        Need r;
-        r.lens = max(p.lens[i], 0);
-        const int64_t pages = (r.lens + n + page - 1) >> p.page_shift;
-        r.held = holds[i];
-        r.need = static_cast<int>(min(pages, static_cast<int64_t>(p.width)));
-        r.over = pages - r.need;
-        return r;
-    };
+    auto pages_of = [&](int i, int n) { return (static_cast<int64_t>(lens[i]) + n + page - 1) >> p.page_shift; };
+    auto need_of = [&](int i) { return Need{holds[i], static_cast<int>(min(pages_of(i, starts[i + 1] - starts[i]), static_cast<int64_t>(p.width)))}; };
     // every CTA goes over all requests: starts, and how many pages come back and go out in front of each
-    int64_t tokens = 0;
-    Sums pages = {0, 0, 0};
+    Saturated tokens = {};
+    Pair pages = {};
     for (int base = 0; base < p.batch; base += kPlanThreads) {
         const int i = base + tid;
         const bool here = i < p.batch;
-        Sums all;
-        const int64_t n_given = here ? max(p.new_lens[i], 0) : 0;
-        const int64_t first = min(tokens + block_before({n_given, 0, 0}, &all, warp_sums).a, static_cast<int64_t>(p.total));
-        const int n = static_cast<int>(min(n_given, p.total - first));
-        tokens += all.a;
-        Sums v = {0, 0, 0};
+        const int n_given = here ? min(max(p.new_lens[i], 0), kCeiling) : 0, cached = here ? max(p.lens[i], 0) : 0, held = here ? min(max(p.held[i], 0), p.width) : 0;
+        Saturated front;
+        const Saturated all = block_before(Saturated{n_given}, &front, token_sums);
+        const int first = min((tokens + front).v, p.total), n = min(n_given, p.total - first);
+        tokens = tokens + all;
+        Pair v = {};
         if (here) {
-            holds[i] = min(max(p.held[i], 0), p.width);
-            const Need r = need_of(i, n);
-            v = {max(r.held - r.need, 0), max(r.need - r.held, 0), r.over};
+            starts[i] = first, lens[i] = cached, holds[i] = held;
+            const int64_t want = pages_of(i, n);
+            const int need = static_cast<int>(min(want, static_cast<int64_t>(p.width)));
+            v = {max(held - need, 0), max(need - held, 0)};
+            if (want > need) atomicAdd(&over, static_cast<unsigned long long>(want - need));
         }
-        const Sums before = block_before(v, &all, warp_sums);
-        if (here) {
-            starts[i] = static_cast<int32_t>(first);
-            back_at[i] = static_cast<int32_t>(pages.a + before.a), want_at[i] = static_cast<int32_t>(pages.b + before.b);
-        }
-        pages.a += all.a, pages.b += all.b, pages.c += all.c;
+        Pair before;
+        const Pair sum = block_before(v, &before, page_sums);
+        if (here) back_at[i] = pages.a + before.a, want_at[i] = pages.b + before.b;
+        pages = pages + sum;
     }
-    if (tid == 0) starts[p.batch] = static_cast<int32_t>(min(tokens, static_cast<int64_t>(p.total)));
+    if (tid == 0) starts[p.batch] = min(tokens.v, p.total);
     const int count = min(max(p.free_count[0], 0), p.capacity);
-    const int there = static_cast<int>(min(count + pages.a, static_cast<int64_t>(p.capacity)));
+    const int there = static_cast<int>(min(static_cast<int64_t>(count) + pages.a, static_cast<int64_t>(p.capacity)));
     __syncthreads();
     // pages that are too many, onto the list: a warp per request
-    for (int i = static_cast<int>(thread / 32); i < p.batch; i += static_cast<int>(threads / 32)) {
-        const Need r = need_of(i, starts[i + 1] - starts[i]);
+    for (int i = thread / 32; i < p.batch; i += threads / 32) {
+        const Need r = need_of(i);
         for (int j = r.need + lane; j < r.held; j += 32) {
             const int64_t at = static_cast<int64_t>(count) + back_at[i] + j - r.need;
             if (at < p.capacity) p.free[at] = p.tables[i * p.table_stride + j];
@@ -122,53 +133,79 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         const int64_t at = static_cast<int64_t>(there) - 1 - (static_cast<int64_t>(want_at[i]) + nth);
         return at >= 0 ? p.free[at] : -1;
     };
-    // positions, slots and ancestors
+    // positions, slots and ancestors: a CTA takes every so many spans of tokens
     const int seen = starts[p.batch];
-    for (int64_t t = thread; t < p.total; t += threads) {
-        int64_t position = -1, slot = -1;
-        uint32_t bits[kMaxWords] = {};
-        if (t < seen) {
-            int lo = 0, hi = p.batch;      // starts[lo] <= t < starts[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (starts[mid] <= t) lo = mid;
-                else hi = mid;
+    for (int64_t span = static_cast<int64_t>(cta) * kSpan; span < p.total; span += static_cast<int64_t>(ctas) * kSpan) {
+        const int base = static_cast<int>(span);
+        if (p.parents) {
+            __syncthreads();      // those of the last span have been read
+            for (int i = tid; i < kSpan + kBehind; i += kPlanThreads) {
+                const int t = base - kBehind + i;
+                family[i] = t >= 0 && t < p.total ? p.parents[t] : -1;
             }
-            const int first = starts[lo], index = static_cast<int>(t) - first;
-            const int64_t lens = max(p.lens[lo], 0), at = lens + index;
-            if (at < room) {
-                const int block = static_cast<int>(at >> p.page_shift), held = holds[lo];
-                const int32_t id = block < held ? p.tables[lo * p.table_stride + block] : page_from(lo, block - held);
-                if (id >= 0) slot = (static_cast<int64_t>(id) << p.page_shift) + (at & (page - 1));
-            }
-            position = at;
-            if (p.parents) {
-                position = lens;
-                // each parent comes before its child, so the walk ends; any other number is no parent
-                for (int node = index;;) {
+            __syncthreads();
+        }
+        int request[kTokens];
 #pragma unroll
-                    for (int w = 0; w < kMaxWords; ++w)
-                        if (w == node >> 5) bits[w] |= 1u << (node & 31);
-                    const int up = p.parents[first + node];
-                    if (up < 0 || up >= node) break;
-                    node = up;
-                    ++position;
+        for (int k = 0; k < kTokens; ++k) {
+            const int t = base + k * kPlanThreads + tid;
+            int lo = 0, hi = p.batch;      // starts[lo] <= t < starts[hi]
+            if (t < seen)
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (starts[mid] <= t) lo = mid;
+                    else hi = mid;
+                }
+            request[k] = lo;
+        }
+        int32_t id[kTokens];
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+            const int t = base + k * kPlanThreads + tid;
+            id[k] = -1;
+            if (t >= seen) continue;
+            const int64_t at = static_cast<int64_t>(lens[request[k]]) + t - starts[request[k]];
+            if (at >= room) continue;
+            const int block = static_cast<int>(at >> p.page_shift), held = holds[request[k]];
+            id[k] = block < held ? p.tables[request[k] * p.table_stride + block] : page_from(request[k], block - held);
+        }
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+            const int t = base + k * kPlanThreads + tid;
+            if (t >= p.total) continue;
+            int64_t position = -1, slot = -1;
+            uint32_t bits[kMaxWords] = {};
+            if (t < seen) {
+                const int first = starts[request[k]], index = t - first;
+                position = static_cast<int64_t>(lens[request[k]]) + index;
+                if (id[k] >= 0) slot = (static_cast<int64_t>(id[k]) << p.page_shift) + (position & (page - 1));
+                if (p.parents) {
+                    position = lens[request[k]];
+                    // each parent comes before its child, so the walk ends; any other number is no parent
+                    for (int node = index;;) {
+#pragma unroll
+                        for (int w = 0; w < kMaxWords; ++w)
+                            if (w == node >> 5) bits[w] |= 1u << (node & 31);
+                        const int at = first + node - base + kBehind, up = at >= 0 ? family[at] : p.parents[first + node];
+                        if (up < 0 || up >= node) break;
+                        node = up;
+                        ++position;
+                    }
                 }
             }
-        }
-        p.positions[t] = position;
-        p.slots[t] = slot;
-        if (p.masks)
+            p.positions[t] = position;
+            p.slots[t] = slot;
+            if (p.masks)
 #pragma unroll
-            for (int w = 0; w < kMaxWords; ++w)
-                if (w < p.words) p.masks[t * p.words + w] = static_cast<int32_t>(bits[w]);
+                for (int w = 0; w < kMaxWords; ++w)
+                    if (w < p.words) p.masks[static_cast<int64_t>(t) * p.words + w] = static_cast<int32_t>(bits[w]);
+        }
     }
     // the tables' new ends and what the requests hold
-    for (int i = static_cast<int>(thread / 32); i < p.batch; i += static_cast<int>(threads / 32)) {
-        const Need r = need_of(i, starts[i + 1] - starts[i]);
+    for (int i = thread / 32; i < p.batch; i += threads / 32) {
+        const Need r = need_of(i);
         const int want = max(r.need - r.held, 0);
         for (int j = lane; j < want; j += 32) p.tables[i * p.table_stride + r.held + j] = page_from(i, j);
-        __syncwarp();
         if (lane == 0) {
             p.held_out[i] = min(r.held, r.need) + min(want, max(there - want_at[i], 0));
             p.starts[i] = starts[i];
@@ -176,9 +213,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     if (thread == 0) {
         p.starts[p.batch] = seen;
-        const int64_t left = max(there - pages.b, static_cast<int64_t>(0));
-        p.free_count_out[0] = static_cast<int32_t>(left);
-        p.free_count_out[1] = static_cast<int32_t>(min(pages.b - (there - left) + pages.c, static_cast<int64_t>(0x7fffffff)));
+        const int left = max(there - pages.b, 0);
+        p.free_count_out[0] = left;
+        p.free_count_out[1] = static_cast<int>(min(static_cast<int64_t>(pages.b) - (there - left) + static_cast<int64_t>(over), static_cast<int64_t>(0x7fffffff)));
     }
 }
 
@@ -249,7 +286,7 @@ bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 }  // namespace
 
 cudaError_t paged_ops_setup() {
-    return cudaFuncSetAttribute(reinterpret_cast<const void *>(&plan_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * kMaxRequests + 1) * 4);
+    return cudaFuncSetAttribute(reinterpret_cast<const void *>(&plan_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kMaxRequests + 1) * 4);
 }
 
 }  // namespace gpuk
@@ -270,6 +307,7 @@ extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int
     if (!starts || !free_count || !free_count_out || (batch && (!lens || !new_lens || !held || !held_out || (table_width && !tables))) || (free_capacity && !free_pages) ||
         (total && (!positions || !slots)))
         return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_plan: null pointer");
+    if (total > kCeiling) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_plan: %d tokens are too many", total);
     const DecodeDevice *d = nullptr;
     const int rc = decode_device(&d);
     if (rc != GPUK_OK) return rc;
@@ -278,7 +316,7 @@ extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int
     int ctas = 1;
     while (ctas < 8 && total > ctas * kPlanThreads) ctas *= 2;
     void *args[] = {&p};
-    const cudaError_t e = launch_kernel(reinterpret_cast<const void *>(&plan_kernel), ctas, kPlanThreads, ctas, false, args, static_cast<cudaStream_t>(stream), (4 * batch + 1) * 4);
+    const cudaError_t e = launch_kernel(reinterpret_cast<const void *>(&plan_kernel), ctas, kPlanThreads, ctas, false, args, static_cast<cudaStream_t>(stream), (5 * batch + 1) * 4);
     if (e != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_plan: launch failed: %s", cudaGetErrorString(e));
     return GPUK_OK;
 }

@@ -187,7 +187,7 @@ def test_roles_meet(slots):
 
 
 # ---- the line of tiles ------------------------------------------------------------------------------------------------
-KEYS, COST, GRAIN, PER_CTA = 64, 256, 384, 256
+KEYS, COST, FRONT, GRAIN, PER_CTA = 64, 256, 192, 128, 256
 
 
 def _share(requests, kv_heads, tile_tokens, masks, room, grid, may_split=True):
@@ -215,7 +215,7 @@ def _share(requests, kv_heads, tile_tokens, masks, room, grid, may_split=True):
     ctas = min(grid, 2 * sum(r[2] for r in reqs) * kv_heads + total // PER_CTA)
 
     def border(c):
-        raw, base = total * c // ctas, 0
+        raw, base = min(total, c * (int(total * 1.00001 / ctas) + 1)), 0
         for i, r in enumerate(reqs):
             head = before(r, r[2])
             if raw >= base + head * kv_heads:
@@ -226,7 +226,7 @@ def _share(requests, kv_heads, tile_tokens, masks, room, grid, may_split=True):
             tile = max(k for k in range(r[2]) if before(r, k) <= at)
             first, last = before(r, tile), before(r, tile + 1)
             pos = at - first
-            if not may_split or r[3] or pos < GRAIN:
+            if not may_split or r[3] or pos < COST + FRONT:
                 pos = 0
             elif last - first - pos < GRAIN:
                 pos = last - first
