@@ -94,6 +94,26 @@ Tensor heads_out(PyObject *o, const Tensor &like, const char *what) {
     return t;
 }
 
+// Contiguous tensors of several sizes and types from one allocation: a call to the allocator for each is what a plan would cost the host most.
+class Pool {
+    int64_t bytes_ = 0;
+    c10::Storage storage_;
+
+  public:
+    int64_t add(int64_t elements, int64_t element_size) {
+        const int64_t at = bytes_;
+        bytes_ += (elements * element_size + 15) / 16 * 16;
+        return at / element_size;      // 16 is a multiple of it
+    }
+    void allocate(const Tensor &like) { storage_ = empty_like_on(like, {std::max<int64_t>(bytes_, 1)}, at::kByte).storage(); }
+    Tensor take(int64_t offset, at::IntArrayRef sizes, at::ScalarType type) const {
+        Tensor t = at::detail::make_tensor<at::TensorImpl>(c10::Storage(storage_), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        t.unsafeGetTensorImpl()->set_storage_offset(offset);
+        return t;
+    }
+};
+
 }  // namespace
 
 // paged_plan(lens, new_lens, tables, held, free, free_count, page_size, total, parents or None, max_new, held_out or None, free_count_out or None)
@@ -138,12 +158,15 @@ PyObject *paged_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
         NoGil unlocked;
         c10::cuda::CUDAGuard guard(lens.device());
         const int rows = int_size(total);
-        if (!held_out.defined()) held_out = empty_like_on(lens, {batch}, at::kInt);
-        if (!count_out.defined()) count_out = empty_like_on(lens, {2}, at::kInt);
-        starts = empty_like_on(lens, {batch + 1}, at::kInt);
-        Tensor both = empty_like_on(lens, {2, total}, at::kLong);
-        positions = both.select(0, 0), slots = both.select(0, 1);
-        if (tree) masks = empty_like_on(lens, {total, words}, at::kInt);
+        Pool pool;
+        const int64_t at_positions = pool.add(total, 8), at_slots = pool.add(total, 8), at_masks = pool.add(total * words, 4), at_starts = pool.add(batch + 1, 4),
+                      at_held = pool.add(batch, 4), at_count = pool.add(2, 4);
+        pool.allocate(lens);
+        if (!held_out.defined()) held_out = pool.take(at_held, {batch}, at::kInt);
+        if (!count_out.defined()) count_out = pool.take(at_count, {2}, at::kInt);
+        starts = pool.take(at_starts, {batch + 1}, at::kInt);
+        positions = pool.take(at_positions, {total}, at::kLong), slots = pool.take(at_slots, {total}, at::kLong);
+        if (tree) masks = pool.take(at_masks, {total, words}, at::kInt);
         check(gpuk_paged_plan(lens.data_ptr<int>(), fresh.data_ptr<int>(), tables.data_ptr<int>(), tables.size(0) > 1 ? tables.stride(0) : tables.size(1), int_size(tables.size(1)),
                               held.data_ptr<int>(), free.data_ptr<int>(), int_size(free.numel()), count.data_ptr<int>(), tree ? parents->data_ptr<int>() : nullptr, int_size(batch), rows,
                               int_size(page), words, starts.data_ptr<int>(), positions.data_ptr<int64_t>(), slots.data_ptr<int64_t>(), tree ? masks.data_ptr<int>() : nullptr,

@@ -70,14 +70,40 @@ __device__ V block_before(V v, V *before, V (&warp_sums)[kPlanWarps + 1]) {
     return all;
 }
 
-// Tokens a thread places at a time, and the parents that its CTA keeps at hand for them: those of the tokens, and of the request that goes on from in front of them.
-constexpr int kTokens = 2, kSpan = kTokens * kPlanThreads, kBehind = 256;
+// Parents that a CTA keeps at hand beside those of its tokens: of the request that goes on from in front of them.
+constexpr int kBehind = 256;
+constexpr int kPlanCtas = 16;      // of a cluster
 
+// The mask of a token: `WORDS` words of 32 bits, two of them as one of 64, none without parents.
+template <int WORDS>
+struct Mask {
+    uint32_t w[WORDS] = {};
+    __device__ void add(int node) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i)
+            if (i == node >> 5) w[i] |= 1u << (node & 31);
+    }
+    __device__ uint32_t word(int i) const { return w[i]; }
+};
+template <>
+struct Mask<0> {
+    __device__ void add(int) {}
+    __device__ uint32_t word(int) const { return 0; }
+};
+template <>
+struct Mask<2> {
+    uint64_t w = 0;
+    __device__ void add(int node) { w |= node < 64 ? 1ull << node : 0ull; }
+    __device__ uint32_t word(int i) const { return static_cast<uint32_t>(w >> 32 * i); }
+};
+
+template <int WORDS>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams p) {
+    constexpr int kTokens = WORDS ? 2 : 4, kSpan = kTokens * kPlanThreads;      // that a thread places at a time, and a CTA
     extern __shared__ int32_t lists[];      // per request: first token, cached tokens, the pages in front that come back or go out, and those that it holds
     __shared__ Saturated token_sums[kPlanWarps + 1];
     __shared__ Pair page_sums[kPlanWarps + 1];
-    __shared__ int32_t family[kSpan + kBehind];
+    __shared__ int32_t family[WORDS ? kSpan + kBehind : 1];
     __shared__ unsigned long long over;      // pages for which the rows of the table have no room
     int32_t *const starts = lists, *const lens = starts + p.batch + 1, *const back_at = lens + p.batch, *const want_at = back_at + p.batch, *const holds = want_at + p.batch;
     const int ctas = cluster_size(), cta = cluster_cta_rank(), tid = threadIdx.x, lane = tid & 31;
@@ -86,6 +112,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     grid_dependency_sync();
     const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
     const int page = 1 << p.page_shift;
+    auto stage_family = [&](int base) {
+        if (WORDS == 0) return;
+#pragma unroll
+        for (int i = 0; i < (kSpan + kBehind + kPlanThreads - 1) / kPlanThreads; ++i) {
+            const int at = i * kPlanThreads + tid, t = base - kBehind + at;
+            if (at < kSpan + kBehind) family[at] = t >= 0 && t < p.total ? p.parents[t] : -1;
+        }
+    };
+    stage_family(cta * kSpan);
 
     struct Need {
         int held, need;
@@ -128,36 +163,30 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
             if (at < p.capacity) p.free[at] = p.tables[i * p.table_stride + j];
         }
     }
-    cluster_barrier();      // the list is whole, and everybody has read the counts: they may be written where they came from
+    cluster_arrive();
     auto page_from = [&](int i, int nth) {
         const int64_t at = static_cast<int64_t>(there) - 1 - (static_cast<int64_t>(want_at[i]) + nth);
         return at >= 0 ? p.free[at] : -1;
     };
     // positions, slots and ancestors: a CTA takes every so many spans of tokens
     const int seen = starts[p.batch];
+    int top = 1;
+    while (top * 2 < p.batch) top *= 2;
+    bool met = false;
     for (int64_t span = static_cast<int64_t>(cta) * kSpan; span < p.total; span += static_cast<int64_t>(ctas) * kSpan) {
         const int base = static_cast<int>(span);
-        if (p.parents) {
+        if (met) {
             __syncthreads();      // those of the last span have been read
-            for (int i = tid; i < kSpan + kBehind; i += kPlanThreads) {
-                const int t = base - kBehind + i;
-                family[i] = t >= 0 && t < p.total ? p.parents[t] : -1;
-            }
+            stage_family(base);
             __syncthreads();
         }
-        int request[kTokens];
+        int request[kTokens] = {};      // the last whose first token is not behind
+        for (int step = top; step > 0; step >>= 1)
 #pragma unroll
-        for (int k = 0; k < kTokens; ++k) {
-            const int t = base + k * kPlanThreads + tid;
-            int lo = 0, hi = p.batch;      // starts[lo] <= t < starts[hi]
-            if (t < seen)
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (starts[mid] <= t) lo = mid;
-                    else hi = mid;
-                }
-            request[k] = lo;
-        }
+            for (int k = 0; k < kTokens; ++k)
+                if (request[k] + step < p.batch && starts[request[k] + step] <= base + k * kPlanThreads + tid) request[k] += step;
+        if (!met) cluster_wait();      // the list is whole, and everybody has read the counts: they may be written where they came from
+        met = true;
         int32_t id[kTokens];
 #pragma unroll
         for (int k = 0; k < kTokens; ++k) {
@@ -174,33 +203,34 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
             const int t = base + k * kPlanThreads + tid;
             if (t >= p.total) continue;
             int64_t position = -1, slot = -1;
-            uint32_t bits[kMaxWords] = {};
+            Mask<WORDS> mask;
             if (t < seen) {
                 const int first = starts[request[k]], index = t - first;
                 position = static_cast<int64_t>(lens[request[k]]) + index;
                 if (id[k] >= 0) slot = (static_cast<int64_t>(id[k]) << p.page_shift) + (position & (page - 1));
-                if (p.parents) {
-                    position = lens[request[k]];
+                if (WORDS) {
                     // each parent comes before its child, so the walk ends; any other number is no parent
+                    const int at = first - base + kBehind;
+                    int depth = 0;
                     for (int node = index;;) {
-#pragma unroll
-                        for (int w = 0; w < kMaxWords; ++w)
-                            if (w == node >> 5) bits[w] |= 1u << (node & 31);
-                        const int at = first + node - base + kBehind, up = at >= 0 ? family[at] : p.parents[first + node];
+                        mask.add(node);
+                        const int up = at + node >= 0 ? family[at + node] : p.parents[first + node];
                         if (up < 0 || up >= node) break;
                         node = up;
-                        ++position;
+                        ++depth;
                     }
+                    position = static_cast<int64_t>(lens[request[k]]) + depth;
                 }
             }
             p.positions[t] = position;
             p.slots[t] = slot;
-            if (p.masks)
+            if (WORDS)
 #pragma unroll
-                for (int w = 0; w < kMaxWords; ++w)
-                    if (w < p.words) p.masks[static_cast<int64_t>(t) * p.words + w] = static_cast<int32_t>(bits[w]);
+                for (int w = 0; w < WORDS; ++w)
+                    if (w < p.words) p.masks[static_cast<int64_t>(t) * p.words + w] = static_cast<int32_t>(mask.word(w));
         }
     }
+    if (!met) cluster_wait();
     // the tables' new ends and what the requests hold
     for (int i = thread / 32; i < p.batch; i += threads / 32) {
         const Need r = need_of(i);
@@ -276,6 +306,11 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const __grid_constan
     if (blockIdx.y == 0 && vec == 0) p.lens_out[request] = static_cast<int32_t>(min(lens + count, static_cast<int64_t>(0x7fffffff)));
 }
 
+// No trees, those of up to 64 nodes, and larger ones.
+const void *plan_of(int words) {
+    if (words == 0) return reinterpret_cast<const void *>(&plan_kernel<0>);
+    return words <= 2 ? reinterpret_cast<const void *>(&plan_kernel<2>) : reinterpret_cast<const void *>(&plan_kernel<kMaxWords>);
+}
 int page_shift_of(int page_size) {
     int s = 0;
     while ((1 << s) < page_size) ++s;
@@ -286,7 +321,12 @@ bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 }  // namespace
 
 cudaError_t paged_ops_setup() {
-    return cudaFuncSetAttribute(reinterpret_cast<const void *>(&plan_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kMaxRequests + 1) * 4);
+    cudaError_t e = cudaSuccess;
+    for (int words : {0, 2, kMaxWords}) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_of(words), cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kMaxRequests + 1) * 4);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_of(words), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    }
+    return e;
 }
 
 }  // namespace gpuk
@@ -314,9 +354,9 @@ extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int
     PlanParams p = {lens, new_lens, held, free_count, parents, tables, free_pages, starts, masks, held_out, free_count_out, positions, slots, table_stride, batch, table_width,
                     page_shift_of(page_size), free_capacity, total, mask_words};
     int ctas = 1;
-    while (ctas < 8 && total > ctas * kPlanThreads) ctas *= 2;
+    while (ctas < kPlanCtas && total > ctas * kPlanThreads) ctas *= 2;
     void *args[] = {&p};
-    const cudaError_t e = launch_kernel(reinterpret_cast<const void *>(&plan_kernel), ctas, kPlanThreads, ctas, false, args, static_cast<cudaStream_t>(stream), (5 * batch + 1) * 4);
+    const cudaError_t e = launch_kernel(plan_of(masks ? mask_words : 0), ctas, kPlanThreads, ctas, false, args, static_cast<cudaStream_t>(stream), (5 * batch + 1) * 4);
     if (e != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_plan: launch failed: %s", cudaGetErrorString(e));
     return GPUK_OK;
 }
