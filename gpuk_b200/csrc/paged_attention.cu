@@ -222,15 +222,13 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
     const int64_t upto = warp_scan(weight, lane), all = __shfl_sync(0xffffffffu, upto, 31), before = upto - weight;
     // enough borders for each tile to have a CTA of its own where there are few
     const int few = __reduce_add_sync(0xffffffffu, static_cast<int>(min(tiles, static_cast<int64_t>(1 << 20))));
-    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), 2 * few + all / kPerCta));
+    const int ctas = static_cast<int>(max(min(static_cast<int64_t>(gridDim.x), 2 * few + all / kPerCta), static_cast<int64_t>(1)));
     const int border = static_cast<int>(blockIdx.x) + side;
     const int64_t share = static_cast<int64_t>(static_cast<float>(all) * (1.00001f / ctas)) + 1;      // the last CTA's is a little shorter
     const int64_t raw = min(all, border * share);
-    if (raw >= all) {      // the line's end
-        if (lane == 0) out->x[side] = all, out->ctas = ctas;
-        return;
-    }
-    if (raw < before || raw >= upto) return;
+    if (lane == 0) out->x[side] = all, out->ctas = ctas;      // the line's end, unless a lane below has the border
+    __syncwarp();
+    if (raw >= all || raw < before || raw >= upto) return;
     int64_t base = before;
     for (int i = lo; i < hi; ++i) {
         if (per > 1) r = request_of(p, i);
@@ -256,7 +254,7 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
         if (!p.may_split || r.over || pos < kTileCost + kFront) pos = 0;
         else if (size - pos < kGrain) pos = size;
         else pos = pos / kKeys * kKeys;      // the borders of blocks, behind the tile's cost
-        out->x[side] = base + kvh * head + first + pos, out->ctas = ctas;
+        out->x[side] = base + kvh * head + first + pos;
         if (side == 0) out->r = r, out->request = i, out->kvh = kvh, out->tile = tile, out->pos = pos;
         return;
     }

@@ -17,6 +17,9 @@ row-wise scales: for decode batches of up to 32 tokens this library's own weight
 otherwise ``torch._scaled_mm`` (a library GEMM; ``own_fp8_gemm=False`` uses libraries everywhere).  Both give the same results to
 within one bf16 step.
 
+``TPDecoder.forward`` has one row of positions per sequence, all at the same ones, as the reference does; ``TPDecoder.forward_paged`` takes requests of any lengths, and
+trees of drafted tokens, over a paged cache (``gpuk_b200/paged.py``).
+
 ``fused=False`` runs the reference arrangement on the same weights -- NCCL ``all_reduce``, then
 add, RMSNorm (and quantisation) as separate PyTorch operators -- and is the comparison arm.
 
@@ -53,6 +56,7 @@ class DecoderArgs:
     norm_eps: float = 1e-6
     rope_theta: float = 500000.0
     dtype: torch.dtype = torch.bfloat16
+    rope_scaling: Optional[dict] = None      # gpuk_b200.paged.scaled_frequencies
 
 
 def _shard_rows(master: torch.Tensor, rank: int, world: int) -> torch.Tensor:
@@ -166,9 +170,12 @@ class TPDecoder:
         norm_gen = torch.Generator(device="cpu").manual_seed(seed * 1000 + 9)
         self.norm = (1 + 0.1 * torch.randn(a.dim, generator=norm_gen)).to(a.dtype).to(self.device)
         self.output = _Linear(make(a.vocab_size, a.dim, 2, "rows"), fp8, own_fp8_gemm)
-        inv = 1.0 / (a.rope_theta ** (torch.arange(0, hd, 2, dtype=torch.int64).float() / hd))   # :497-502
-        freqs = torch.outer(torch.arange(a.max_seq_len * 2, dtype=torch.float32), inv)
-        self.cos, self.sin = freqs.cos().to(self.device), freqs.sin().to(self.device)
+        inv, amplitude = 1.0 / (a.rope_theta ** (torch.arange(0, hd, 2, dtype=torch.int64).float() / hd)), 1.0   # :497-502
+        if a.rope_scaling is not None:
+            inv, amplitude = gpuk.paged.scaled_frequencies(hd, a.rope_theta, a.rope_scaling)
+        freqs = torch.outer(torch.arange(a.max_seq_len * 2, dtype=inv.dtype), inv)
+        self.cos, self.sin = ((f * amplitude).float().to(self.device) for f in (freqs.cos(), freqs.sin()))
+        self.frequencies = None      # the same for positions in a paged cache, once it is used
         self._zeros = {}
         # the elementwise steps between the projections as this library's kernels (csrc/decoder_ops.cu)
         self.own_elementwise = fused and self.device.type == "cuda" and a.dtype == torch.bfloat16 and hd % 16 == 0 and a.ffn_dim // w % 8 == 0
@@ -191,13 +198,15 @@ class TPDecoder:
         cos, sin = cos.unsqueeze(-2), sin.unsqueeze(-2)
         return torch.cat((x1 * cos - x2 * sin, x2 * cos + x1 * sin), dim=-1).type_as(x)
 
-    def _norm_only(self, h: torch.Tensor, weight: torch.Tensor):
+    def _norm_only(self, h: torch.Tensor, weight: torch.Tensor, keep: bool = True):
         """RMSNorm (+ FP8) of the embeddings before the first layer: the fused operator with a
-        zero residual on this rank alone."""
+        zero residual on this rank alone, kept for the next call of the same shape."""
         if self.fused:
             z = self._zeros.get(h.shape)
             if z is None:
-                z = self._zeros[h.shape] = torch.zeros_like(h)
+                z = torch.zeros_like(h)
+                if keep:
+                    self._zeros[h.shape] = z
             results = _native.add_rms(0, h, z, weight, self.args.norm_eps, 3 if self.fp8 else 0, None)
             if results is not None:
                 return results[1], results[2] if self.fp8 else None
@@ -265,7 +274,7 @@ class TPDecoder:
         tables = mask = None      # what the operators need, once one of them is called
         normed, scale = self._norm_only(h, self.layers[0]["attention_norm"])
         for li, layer in enumerate(self.layers):
-            q = att = act = None      # a native call returns None where the operators are wanted
+            q = att = None      # a native call returns None where the operators are wanted
             fused = layer["wqkv"].streamed(normed) if own and hd == 128 else None
             if fused is not None:
                 q = _native.qkv_rope(normed, scale, *fused, self.cos, self.sin, pos, layer["k_cache"], layer["v_cache"], self.h_local)
@@ -297,19 +306,54 @@ class TPDecoder:
                         mask = mask | (input_pos < -a.max_seq_len)[:, None]      # a token that the rotary embedding marked attends, and stays marked
                 att = F.scaled_dot_product_attention(q.transpose(1, 2), layer["k_cache"][:b, :, :last], layer["v_cache"][:b, :, :last],
                                                      attn_mask=mask, enable_gqa=True).transpose(1, 2).reshape(b * t, self.h_local * hd)
-            partial = layer["wo"](att)
-            h, normed, scale = self._reduce_add_norm(partial, h, layer["ffn_norm"])
-            fused = layer["w13"].streamed(normed) if own else None
-            if fused is not None:
-                act = _native.swiglu(normed, scale, *fused)
-            if act is None:
-                f13 = layer["w13"](normed, scale)
-                if own:
-                    act = _native.silu_mul(f13)
-            if act is None:
-                f1, f3 = f13.split(a.ffn_dim // self.world, dim=-1)
-                act = F.silu(f1) * f3
-            partial = layer["w2"](act)
-            nxt = self.layers[li + 1]["attention_norm"] if li + 1 < a.n_layers else self.norm
-            h, normed, scale = self._reduce_add_norm(partial, h, nxt)
+            h, normed, scale = self._after_attention(li, att, h, own)
         return self.output(normed, scale).view(b, t, -1)
+
+    def _after_attention(self, li: int, att: torch.Tensor, h: torch.Tensor, own: bool):
+        """From a layer's attention to the input of the next layer's projections."""
+        a, layer = self.args, self.layers[li]
+        act = None      # a native call returns None where the operators are wanted
+        partial = layer["wo"](att)
+        h, normed, scale = self._reduce_add_norm(partial, h, layer["ffn_norm"])
+        fused = layer["w13"].streamed(normed) if own else None
+        if fused is not None:
+            act = _native.swiglu(normed, scale, *fused)
+        if act is None:
+            f13 = layer["w13"](normed, scale)
+            if own:
+                act = _native.silu_mul(f13)
+        if act is None:
+            f1, f3 = f13.split(a.ffn_dim // self.world, dim=-1)
+            act = F.silu(f1) * f3
+        partial = layer["w2"](act)
+        nxt = self.layers[li + 1]["attention_norm"] if li + 1 < a.n_layers else self.norm
+        return self._reduce_add_norm(partial, h, nxt)
+
+    def paged_cache(self, pages: int, requests: int, pages_per_request: int, page_size: int = 64) -> gpuk.PagedKVCache:
+        """An empty cache of this rank's KV heads for ``forward_paged``."""
+        a = self.args
+        return gpuk.PagedKVCache(a.n_layers, pages, page_size, self.kv_local, a.head_dim, requests, pages_per_request, dtype=a.dtype, device=self.device)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, cache: gpuk.PagedKVCache, plan: gpuk.PagedPlan, max_len: Optional[int] = None) -> torch.Tensor:
+        """tokens [total], the new ones of all requests one after another as ``plan`` (``cache.plan``) has them -> logits [total, vocab/world] of this rank's vocabulary
+        shard.  Requests may be of any lengths and have any number of new tokens: one each, a tree of drafts to be verified, a prompt.  Their keys and values are in the
+        cache's pages afterwards, and count from ``cache.append`` or ``cache.keep`` on.  Logits of a token without a slot are NaN; those of rows behind the last request
+        mean nothing.  ``max_len``: no request has more cached and new tokens.  Heads of 64 or 128; there is no CPU path."""
+        a = self.args
+        if self.device.type != "cuda":
+            raise RuntimeError("gpuk: a paged cache needs a CUDA device")
+        if tokens.shape != plan.positions.shape:
+            raise RuntimeError(f"gpuk: {tuple(tokens.shape)} tokens for a plan of {plan.positions.shape[0]}")
+        if self.frequencies is None:
+            self.frequencies = gpuk.rope_frequencies(a.head_dim, a.rope_theta, scaling=a.rope_scaling, device=self.device)
+        hd, heads = a.head_dim, [self.h_local, self.kv_local, self.kv_local]
+        h = F.embedding(tokens, self.tok_embeddings)
+        normed, scale = self._norm_only(h, self.layers[0]["attention_norm"], keep=False)      # ragged batches have any number of rows
+        for li, layer in enumerate(self.layers):
+            k_pages, v_pages = cache.k[li], cache.v[li]
+            q, k, v = layer["wqkv"](normed, scale).view(-1, sum(heads), hd).split(heads, dim=1)
+            q = gpuk.rope_paged(q, k, v, plan.positions, plan.slots, self.frequencies, k_pages, v_pages, layout="split")
+            att = gpuk.paged_attention(q, k_pages, v_pages, cache.tables, cache.lens, plan.starts, masks=plan.masks, max_len=max_len)
+            h, normed, scale = self._after_attention(li, att.view(-1, self.h_local * hd), h, self.own_elementwise)
+        return self.output(normed, scale)
