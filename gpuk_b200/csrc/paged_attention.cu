@@ -154,13 +154,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Barriers by their address in shared memory: the single threads that copy and multiply are bound by the instructions between two waits.
+// A wait gives up after some two seconds.
 __device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity) {
-    for (uint32_t spin = 0; spin < (1u << 24); ++spin) {
+    uint64_t began = 0;
+    for (uint32_t spin = 1;; ++spin) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
+        if (spin % 1024 == 0) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (began == 0) began = now;
+            else if (now - began > 2000000000ull) return false;
+        }
     }
-    return false;
 }
 __device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
@@ -308,7 +315,8 @@ __device__ __forceinline__ uint64_t seen_of(const PagedAttentionParams &p, const
     const uint64_t cached = old == kKeys ? ~0ull : (1ull << old) - 1;
     if (old == kKeys) return cached;
     const int rel = base + old - u.ctx;
-    const int most = min(p.masks ? u.n - rel : tok + 1 - rel, kKeys - old);
+    const int room = static_cast<int>(min(room_of(p) - base - old, static_cast<int64_t>(kKeys - old)));      // tokens behind the table's row have no keys
+    const int most = min(p.masks ? u.n - rel : tok + 1 - rel, room);
     uint64_t fresh = most <= 0 ? 0 : most == 64 ? ~0ull : (1ull << most) - 1;
     if (p.masks && fresh) fresh &= mask_bits(p.masks + static_cast<int64_t>(u.start + tok) * p.words, p.words, rel);
     return cached | fresh << old;

@@ -39,6 +39,7 @@ struct RopeParams {
     float amplitude;
     int tokens, heads, kv_heads, head_dim, rotary, page_shift, layout;
     int chunks, chunk_items;      // CTAs a token, items of each
+    int streaming;                // more is written than L2 keeps until it is read
     int *status;
 };
 
@@ -130,8 +131,13 @@ __global__ void rope_kernel(const __grid_constant__ RopeParams p) {
             dst = static_cast<T *>(key ? p.k_pages : p.v_pages) + (slot >> p.page_shift) * p.page_stride + (key ? kv : kv - p.kv_heads) * p.head_stride +
                   (slot & ((1 << p.page_shift) - 1)) * p.row_stride;
         }
-        *reinterpret_cast<uint4 *>(dst + c) = lo;
-        *reinterpret_cast<uint4 *>(dst + d) = hi;
+        if (p.streaming) {
+            __stcs(reinterpret_cast<uint4 *>(dst + c), lo);
+            __stcs(reinterpret_cast<uint4 *>(dst + d), hi);
+        } else {
+            *reinterpret_cast<uint4 *>(dst + c) = lo;
+            *reinterpret_cast<uint4 *>(dst + d) = hi;
+        }
     }
     if (!there && slot >= 0 && threadIdx.x == 0) *p.status = 1;
 }
@@ -160,6 +166,8 @@ int launch(RopeParams &p, int dtype, void *stream, const char *what) {
     if (chunks < least) chunks = least;
     p.chunk_items = static_cast<int>((items + chunks - 1) / chunks);
     p.chunks = static_cast<int>((items + p.chunk_items - 1) / p.chunk_items);
+    // 8191 tokens of 64 + 16 heads of 128: 59.4 us, 62.5 with stores that stay in L2; a step of a few tokens is read from there by the attention behind it
+    p.streaming = p.tokens * items * (kVec * 2) > 64ll << 20;
     const int threads = (p.chunk_items + kItems - 1) / kItems;
     if (static_cast<int64_t>(p.tokens) * p.chunks > 0x7fffffffll) return set_last_error(GPUK_ERR_UNSUPPORTED, "%s: too many tokens", what);
     const void *fn = dtype == GPUK_DTYPE_BF16 ? reinterpret_cast<const void *>(&rope_kernel<__nv_bfloat16>) : reinterpret_cast<const void *>(&rope_kernel<__half>);

@@ -384,9 +384,9 @@ int gpuk_decode_attention(const void *q, const void *k_cache, const void *v_cach
 int gpuk_prefill_attention(const void *q, const void *k_cache, const void *v_cache, const int64_t *pos, void *out, int batch, int t, int heads, int kv_heads,
                            int head_dim, int len, int max_seq, void *stream);
 /*
- * Synchronises the current device and returns GPUK_ERR_BAD_LAUNCH if a launch of one of the calls above on it
+ * Synchronises the current device and returns GPUK_ERR_BAD_LAUNCH if a launch of one of the calls above, or of gpuk_paged_attention, on it
  * found itself in another thread-block cluster than planned (it then wrote nothing) or gave up a wait; GPUK_ERR_INVALID_ARGUMENT, once, if a position
- * given to gpuk_qkv_rope_skinny or gpuk_rope_append lay outside the cache or the table of angles; else GPUK_OK.
+ * given to gpuk_qkv_rope_skinny or gpuk_rope_append lay outside the cache or the table of angles, or a slot given to gpuk_rope_paged behind the pages; else GPUK_OK.
  * Same contract as status 3 of gpuk_ws_status; the reference has no counterpart (impl.h launches no clusters).
  */
 int gpuk_fp8_linear_status(void);

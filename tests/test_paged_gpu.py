@@ -436,6 +436,25 @@ def test_rows_behind_the_last_request_are_left():
     assert torch.equal(out[:41], want) and bool((out[41:] == 3).all())
 
 
+def test_the_bound_on_lengths_is_a_hint():
+    """A smaller one than the lengths, and none: the keys are cut or not, the result is the formula's."""
+    b = _Batch([5000, 1, 700], [3, 200, 9], 16, 2, 128, 32, seed=6)
+    for bound in (None, 0, 1, 319, 320, 10 ** 12):
+        b.check(b.run(max_len=bound))
+
+
+def test_more_tokens_than_the_table_holds():
+    """Those behind the row's end have no keys: they see what there is; nothing is read outside the row."""
+    b = _Batch([16], [40], 4, 2, 64, 16, spare=9)
+    want = gpuk.paged_attention(b.q, b.k, b.v, b.tables[:, :2], b.lens, b.starts)
+    _status_ok()
+    full, b.keys, b.values = b.seen, [k[:32] for k in b.keys], [v[:32] for v in b.values]
+    b.seen = lambda i: full(i)[:, :32]
+    b.check(want)
+    b.seen = lambda i: torch.ones(40, 32, dtype=torch.bool, device="cuda")
+    b.check(gpuk.paged_attention(b.q, b.k, b.v, b.tables[:, :2], _ints([2 ** 31 - 1]), b.starts))
+
+
 def test_many_requests_and_one_long_context():
     """Uneven work: one context is cut into many parts, the others into one; more requests than a warp has lanes."""
     rng = random.Random(2)
