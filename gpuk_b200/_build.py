@@ -27,8 +27,8 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
 ]
 CORE_SOURCES = ["core.cu", "launch_bf16.cu", "launch_f16.cu", "launch_f32.cu", "noalloc.cu", "fp8_linear.cu", "stream_linear.cu", "tensor_map.cu", "decoder_ops.cu",
-                "attention.cu", "prefill_attention.cu", "paged_ops.cu", "paged_attention.cu", "rope.cu"]
-HEADERS = ["common.cuh", "epilogue.cuh", "kernels.cuh", "launch.cuh", "launch_impl.cuh", "linear.cuh", "tensor_core.cuh", "decoder_math.cuh",
+                "attention.cu", "prefill_attention.cu", "paged_ops.cu", "paged_attention.cu", "paged_decode.cu", "rope.cu"]
+HEADERS = ["common.cuh", "epilogue.cuh", "kernels.cuh", "launch.cuh", "launch_impl.cuh", "linear.cuh", "tensor_core.cuh", "decoder_math.cuh", "paged_share.cuh",
            os.path.join(ROOT, "include", "gpuk_b200.h")]
 
 

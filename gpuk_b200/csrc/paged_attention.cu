@@ -18,8 +18,6 @@
 //
 // fp32 scores, maxima, sums and outputs.  Probabilities are rounded to the operands' type for the second product; in fp16 they are held times 2^10, so that small
 // ones do not fall under its smallest numbers.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -28,50 +26,24 @@
 #include "../../include/gpuk_b200.h"
 #include "launch.cuh"
 #include "linear.cuh"
+#include "paged_share.cuh"
 #include "tensor_core.cuh"
 
 namespace gpuk {
 namespace {
 
-constexpr int kRows = 128;                       // of a tile
-constexpr int kKeys = 64;                        // of a block
 constexpr int kThreads = kRows + 64;             // a thread per row, a warp that multiplies, one that copies
 constexpr int kSpanBytes = kKeys * 128;          // 64 rows of one swizzle span (64 values)
 constexpr int kQSpanBytes = kRows * 128;
 constexpr int kColumns = 256;                    // two score buffers of 64, up to 128 of outputs
 constexpr int kOut = 2 * kKeys;                  // first column of the outputs
 constexpr int kMaskedBlocks = 8;                 // that a tile can have
-constexpr int kCtasPerSm = 2;
-constexpr int kTileCost = 4 * kKeys;             // what a tile costs beside its keys, in keys: its queries, its outputs, the first scores
-constexpr int kGrain = 2 * kKeys;                // no tile is cut nearer than that to its end, or than kFront to its beginning
-constexpr int kFront = 3 * kKeys;
-constexpr int kPerCta = 256;                     // keys for which a call takes another CTA
 constexpr int kFewTiles = 4;                     // of a request, whose pages are not kept in L2
 constexpr int kQueue = 4;                        // segments that are described at a time
 
-constexpr float kLowest = -3.4e38f;              // a maximum before any key ...
-constexpr float kSeen = -3.3e38f;                // ... and where all scores are -infinity: finite both, and below any score behind them
 
 template <int HD>
 constexpr int kSlotsOf = HD == 128 ? 5 : 10;
-
-// Blocks [first, first + blocks) of the keys of a tile: what a CTA does at a time.
-struct alignas(16) Segment {
-    int request, start, n, ctx;                  // its first row in q, new and cached tokens
-    int tok0, kvh;                               // the tile's first token
-    int first, blocks;                           // no blocks: the end
-    int slot;                                    // of the partial results; -1: the whole tile
-};
-struct Request {
-    int start, n, ctx, tiles;
-    bool over;      // more tokens than the table's row holds: its tiles are not cut
-};
-// Where a CTA begins: weight `pos` of a tile; and its borders on the line of all tiles.
-struct Start {
-    Request r;
-    int request, kvh, tile, ctas;
-    int64_t pos, x[2];
-};
 
 // A wait tells a phase of a barrier from the one before and the one behind it, not from the next but one.  Scores, products and queries have two barriers in turn, since a row's thread
 // may come to block j when product j - 2 is the last that is known to be complete, and to its end when the last product is.
@@ -86,58 +58,6 @@ struct Smem {
     uint32_t poison[3][kMaskedBlocks * 2];       // keys of the masked blocks with a value that is no finite number, of a segment, the next and the one before
 };
 
-struct PagedAttentionParams {
-    const int32_t *tables, *lens, *starts, *masks;
-    const void *v;
-    void *out;
-    int64_t table_stride, page_stride, head_stride, row_stride, num_pages;
-    int64_t out_token, out_head;
-    int batch, tokens, kv_heads, group, tile_tokens, words;
-    uint32_t tile_inverse;                       // 2^32 / tile_tokens, rounded up
-    int width, page_shift;                       // of a row of the table, and log2 of a page's tokens
-    int may_split, out_sectors;                  // rows of the outputs lie on borders of 32 bytes
-    float scale_log2;
-    int *status;
-    // of the partial results, for `ctas` CTAs: see Joint, [2 * ctas][HD / 4][128][4] outputs (a warp's rows side by side), [2 * ctas][2][128] maxima and sums
-    struct Joint *joints;
-    float *partial, *stats;
-};
-// What the second kernel learns from each CTA of the first.
-struct alignas(16) Joint {
-    Segment open;                                // a tile that begins in the CTA and goes on behind it (slot -1: none)
-    int head;                                    // the CTA takes: 0 nothing, 1 a part of such a tile and nothing else, 2 the last part of one, 3 begins with a tile
-    int ctas;                                    // that take part
-};
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-template <typename T>
-struct Half;
-template <>
-struct Half<__nv_bfloat16> {
-    static constexpr int kFormat = 1;
-    static constexpr uint32_t kExponent = 0x7f807f80u;
-    static constexpr float kBias = 0.f, kLag = 8.f;
-    __device__ static uint32_t pack(float lo, float hi) {
-        uint32_t r;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-        return r;
-    }
-};
-template <>
-struct Half<__half> {
-    static constexpr int kFormat = 0;
-    static constexpr uint32_t kExponent = 0x7c007c00u;
-    static constexpr float kBias = 8.f, kLag = 7.f;      // 2^15 at most
-    __device__ static uint32_t pack(float lo, float hi) {
-        uint32_t r;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-        return r;
-    }
-};
 // Nonzero where one of the two halves is an infinity or NaN: all bits of its exponent are set.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w, uint32_t exponent) {
     const uint32_t x = (w & exponent) ^ exponent;      // a zero half
@@ -181,127 +101,6 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r != 0;
 }
-
-// ---- which parts of which tiles a CTA takes ---------------------------------------------------------
-// Tiles lie one after another, by request, kv head and token, each as long as the keys that it sees and kTileCost more.  A CTA takes an equal share of that line; where a border comes
-// near an end of a tile it goes to that end.
-__device__ __forceinline__ int64_t room_of(const PagedAttentionParams &p) { return static_cast<int64_t>(p.width) << p.page_shift; }
-__device__ __forceinline__ Request request_of(const PagedAttentionParams &p, int i) {
-    Request r;
-    r.start = min(max(p.starts[i], 0), p.tokens);
-    r.n = min(max(p.starts[i + 1], r.start), p.tokens) - r.start;
-    r.ctx = static_cast<int>(min(static_cast<int64_t>(max(p.lens[i], 0)), room_of(p)));
-    r.tiles = static_cast<int>(p.tile_tokens == 1 ? r.n : __umulhi(r.n + p.tile_tokens - 1, p.tile_inverse));      // exact below 2^32 / tile_tokens
-    r.over = static_cast<int64_t>(r.ctx) + r.n > room_of(p);
-    return r;
-}
-// Keys that some row of a tile sees.
-__device__ __forceinline__ int64_t keys_of(const PagedAttentionParams &p, const Request &r, int tile) {
-    const int64_t most = static_cast<int64_t>(r.ctx) + (p.masks ? static_cast<int64_t>(r.n) : min(static_cast<int64_t>(r.n), static_cast<int64_t>(tile + 1) * p.tile_tokens));
-    return min(most, room_of(p));
-}
-// The weight of a tile, and of those in front of one.
-__device__ __forceinline__ int64_t weight_of(const PagedAttentionParams &p, const Request &r, int tile) { return kTileCost + (r.over ? room_of(p) : keys_of(p, r, tile)); }
-__device__ __forceinline__ int64_t weight_before(const PagedAttentionParams &p, const Request &r, int tile) {
-    if (r.tiles == 0) return 0;
-    if (p.masks || r.over) return tile * (kTileCost + min(static_cast<int64_t>(r.ctx) + r.n, room_of(p)));
-    const int64_t whole = min(tile, r.tiles - 1), w = whole * (kTileCost + r.ctx) + p.tile_tokens * (whole * (whole + 1) / 2);
-    return tile < r.tiles || tile == 0 ? w : w + kTileCost + r.ctx + r.n;
-}
-// Sums over the lanes up to this one.
-__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += t;
-    }
-    return v;
-}
-
-// One warp for each of a CTA's two borders; lane l looks after a run of the requests.  Quotients are estimated in fp32 and put right, which is faster than dividing 64 bits.
-__device__ void find_border(const PagedAttentionParams &p, Start *out, int side) {
-    const int lane = threadIdx.x & 31, per = (p.batch + 31) / 32, lo = min(lane * per, p.batch), hi = min(lo + per, p.batch);
-    int64_t weight = 0, tiles = 0;
-    Request r = {};
-    for (int i = lo; i < hi; ++i) {
-        r = request_of(p, i);
-        weight += weight_before(p, r, r.tiles) * p.kv_heads, tiles += static_cast<int64_t>(r.tiles) * p.kv_heads;
-    }
-    const int64_t upto = warp_scan(weight, lane), all = __shfl_sync(0xffffffffu, upto, 31), before = upto - weight;
-    // enough borders for each tile to have a CTA of its own where there are few
-    const int few = __reduce_add_sync(0xffffffffu, static_cast<int>(min(tiles, static_cast<int64_t>(1 << 20))));
-    const int ctas = static_cast<int>(max(min(static_cast<int64_t>(gridDim.x), 2 * few + all / kPerCta), static_cast<int64_t>(1)));
-    const int border = static_cast<int>(blockIdx.x) + side;
-    const int64_t share = static_cast<int64_t>(static_cast<float>(all) * (1.00001f / ctas)) + 1;      // the last CTA's is a little shorter
-    const int64_t raw = min(all, border * share);
-    if (lane == 0) out->x[side] = all, out->ctas = ctas;      // the line's end, unless a lane below has the border
-    __syncwarp();
-    if (raw >= all || raw < before || raw >= upto) return;
-    int64_t base = before;
-    for (int i = lo; i < hi; ++i) {
-        if (per > 1) r = request_of(p, i);
-        const int64_t head = weight_before(p, r, r.tiles), here = head * p.kv_heads;
-        if (raw >= base + here) {
-            base += here;
-            continue;
-        }
-        int64_t at = raw - base, first = 0;
-        int kvh = min(p.kv_heads - 1, static_cast<int>(__fdividef(static_cast<float>(at), static_cast<float>(head)))), tile = 0;
-        while (kvh > 0 && kvh * head > at) --kvh;
-        while (kvh + 1 < p.kv_heads && (kvh + 1) * head <= at) ++kvh;
-        at -= kvh * head;
-        if (r.tiles > 1) {      // weight_before(tile) <= at < weight_before(tile + 1): a line, or a parabola with half a tile's tokens to the square
-            const float slope = kTileCost + r.ctx + (p.masks || r.over ? static_cast<float>(r.n) : 0.5f * p.tile_tokens), bend = p.masks || r.over ? 0.f : 0.5f * p.tile_tokens;
-            tile = min(r.tiles - 1, static_cast<int>(bend == 0.f ? static_cast<float>(at) / slope : (sqrtf(slope * slope + 4.f * bend * at) - slope) / (2.f * bend)));
-            while (tile > 0 && weight_before(p, r, tile) > at) --tile;
-            while (tile + 1 < r.tiles && weight_before(p, r, tile + 1) <= at) ++tile;
-            first = weight_before(p, r, tile);
-        }
-        const int64_t size = weight_of(p, r, tile);
-        int64_t pos = at - first;
-        if (!p.may_split || r.over || pos < kTileCost + kFront) pos = 0;
-        else if (size - pos < kGrain) pos = size;
-        else pos = pos / kKeys * kKeys;      // the borders of blocks, behind the tile's cost
-        out->x[side] = base + kvh * head + first + pos;
-        if (side == 0) out->r = r, out->request = i, out->kvh = kvh, out->tile = tile, out->pos = pos;
-        return;
-    }
-}
-
-// The segments of a CTA one after another.
-struct Walk {
-    Request r;
-    int request, kvh, tile, index;
-    int64_t pos, left;
-    __device__ explicit Walk(const Start &s) : r(s.r), request(s.request), kvh(s.kvh), tile(s.tile), index(0), pos(s.pos), left(s.x[1] - s.x[0]) {}
-    __device__ bool next(const PagedAttentionParams &p, Segment *out, bool *begins, bool *ends) {
-        if (left <= 0) return false;
-        int64_t size = weight_of(p, r, tile);
-        while (pos >= size) {      // at a tile's end, to the next
-            pos = 0;
-            if (++tile >= r.tiles) {
-                tile = 0;
-                if (++kvh >= p.kv_heads) {
-                    kvh = 0;
-                    do {
-                        if (++request >= p.batch) return false;      // cannot be: the weights say that there is more
-                        r = request_of(p, request);
-                    } while (r.tiles == 0);
-                }
-            }
-            size = weight_of(p, r, tile);
-        }
-        const int64_t take = min(size - pos, left), end = pos + take;
-        const int all = static_cast<int>((keys_of(p, r, tile) + kKeys - 1) / kKeys);
-        auto block_at = [&](int64_t w) { return w <= kTileCost ? 0 : static_cast<int>(min((w - kTileCost + kKeys - 1) / kKeys, static_cast<int64_t>(all))); };
-        *begins = pos == 0, *ends = end == size;
-        const int first = *begins ? 0 : block_at(pos), last = *ends ? all : block_at(end);
-        *out = {request, r.start, r.n, r.ctx, tile * p.tile_tokens, kvh, first, last - first, -1};
-        if (!*begins || !*ends) out->slot = 2 * static_cast<int>(blockIdx.x) + (*begins && index > 0);
-        pos = end, left -= take, ++index;
-        return true;
-    }
-};
 
 // Bits [at, at + 64) of a row of mask words, zeros outside.
 __device__ __forceinline__ uint64_t mask_bits(const int32_t *row, int words, int at) {
@@ -694,17 +493,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
 
 // Parts of a tile joined: the one that the CTA where the tile begins left, and those of the CTAs behind it up to the tile's last, in that order.  A CTA takes 32 rows of a tile, a lane
 // for each; its warps read the statistics of as many parts at a time, and then each its share of the values of all parts.
-constexpr int kJoinWarps = 8, kJoinCtas = kRows / 32, kJoinParts = 32;
+constexpr int kJoinWarps = 8, kJoinParts = 32;
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32, 3) join_kernel(const __grid_constant__ PagedAttentionParams p) {
     constexpr int kVecs = HD / 4 / kJoinWarps, kAhead = 8 / kVecs;      // vectors of four that a lane sums up, and parts of them that it reads at a time
     __shared__ float maxima[kJoinParts][32], sums[kJoinParts][32];
     __shared__ int slots[kJoinParts];
     grid_dependency_sync();
-    const int cta = blockIdx.x / kJoinCtas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = p.joints[0].ctas;
+    const int cta = blockIdx.x / p.row_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = p.joints[0].ctas;
     if (cta >= ctas) return;
     const Segment u = p.joints[cta].open;
-    const int row = blockIdx.x % kJoinCtas * 32 + lane, tok = u.tok0 + row / p.group;
+    const int row = blockIdx.x % p.row_groups * 32 + lane, tok = u.tok0 + row / p.group;
     const bool valid = u.slot >= 0 && row < p.tile_tokens * p.group && tok < u.n;
     if (!__any_sync(0xffffffffu, valid)) return;      // the same in all warps
     const float4 *partial = reinterpret_cast<const float4 *>(p.partial) + warp * kVecs * kRows + row;
@@ -775,20 +574,24 @@ struct Shape {
     int group, tile_tokens, may_split;
     int64_t grid, bytes;
 };
-Shape shape_of(int batch, int tokens, int heads, int kv_heads, int head_dim, int64_t max_len, int sms) {
+// `single`: no more new tokens than requests, and so in all likelihood one for each.  Both kernels give the formula's result whatever the requests have; for single tokens the one that is built
+// for them takes 4 x 100 to 300 keys of 16 / 4 heads in 6.6 us instead of 9.7, 32 x 30 to 4000 of 64 / 8 in 39.4 instead of 42.7.
+Shape shape_of(int batch, int tokens, int heads, int kv_heads, int head_dim, int64_t max_len, int sms, bool single) {
     Shape s = {};
     s.group = heads / kv_heads;
-    s.tile_tokens = kRows / s.group;
+    s.tile_tokens = single ? 1 : kRows / s.group;
     // sum of ceil(n / t) <= floor(sum of n / t) + requests with new tokens
     const int64_t full = tokens / s.tile_tokens, some = batch < tokens ? batch : tokens;
     const int64_t tiles = (full + some < tokens ? full + some : tokens) * kv_heads;
     s.may_split = max_len >= kFront + kGrain;      // shorter tiles are never cut
     const int64_t most = static_cast<int64_t>(sms) * kCtasPerSm, want = 2 * tiles + tiles * (max_len + kTileCost) / kPerCta;
-    s.grid = tiles >= most || want >= most ? most : want;
+    s.grid = single && !s.may_split ? tiles : tiles >= most || want >= most ? most : want;
     s.bytes = s.may_split ? s.grid * (static_cast<int64_t>(sizeof(Joint)) + 2ll * kRows * (head_dim + 2) * 4) : 0;
     return s;
 }
 
+int row_groups_of(const Shape &s) { return (s.tile_tokens * s.group + 31) / 32; }
+bool single_tokens(int batch, int tokens, int heads, int kv_heads, bool masks) { return !masks && tokens <= batch && heads / kv_heads <= kDecodeGroup; }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_shape(const gpuk_pages *pages, int batch, int tokens, int heads, int64_t max_len) {
@@ -810,6 +613,9 @@ cudaError_t paged_attention_setup() {
         for (int hd : {64, 128}) {
             const Kernels k = kernels_of(dtype, hd);
             if (e == cudaSuccess) e = cudaFuncSetAttribute(k.attend, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+            int smem = 0;
+            const void *decode = paged_decode_of(dtype, hd, &smem);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(decode, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         }
     return e;
 }
@@ -827,7 +633,12 @@ extern "C" int gpuk_paged_attention_workspace(const gpuk_pages *pages, int batch
     const DecodeDevice *d = nullptr;
     rc = decode_device(&d);
     if (rc != GPUK_OK) return rc;
-    *bytes = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms).bytes;
+    // of the kernel that needs more: which one a call takes depends on its masks too
+    for (bool single : {false, true}) {
+        if (single && !single_tokens(batch, tokens, heads, pages->kv_heads, false)) continue;
+        const int64_t need = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms, single).bytes;
+        if (need > *bytes) *bytes = need;
+    }
     return GPUK_OK;
 }
 
@@ -853,36 +664,46 @@ extern "C" int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64
     const DecodeDevice *d = nullptr;
     rc = decode_device(&d);
     if (rc != GPUK_OK) return rc;
-    Shape s = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms);
+    const bool single = single_tokens(batch, tokens, heads, pages->kv_heads, masks != nullptr);
+    const Shape s = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms, single);
+    if (s.grid * row_groups_of(s) > 0x7fffffffll) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: too many tokens");
     if (s.may_split && (!workspace || workspace_bytes < s.bytes || !aligned16(workspace)))
         return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: needs a workspace of %lld bytes, 16-byte aligned", static_cast<long long>(s.bytes));
     const int hd = pages->head_dim;
-    const CUtensorMapDataType type = pages->dtype == GPUK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUtensorMap qmap, kmap, vmap;
-    const uint64_t q_sizes[3] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
-    const uint64_t q_strides[2] = {static_cast<uint64_t>(q_head_stride) * 2, static_cast<uint64_t>(q_token_stride) * 2};
-    const uint32_t q_box[3] = {64, static_cast<uint32_t>(s.group), static_cast<uint32_t>(s.tile_tokens)};
-    const uint64_t sizes[4] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(p2), static_cast<uint64_t>(pages->kv_heads), static_cast<uint64_t>(pages->num_pages)};
-    const uint64_t strides[3] = {static_cast<uint64_t>(pages->row_stride) * 2, static_cast<uint64_t>(pages->head_stride) * 2, static_cast<uint64_t>(pages->page_stride) * 2};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(p2 < kKeys ? p2 : kKeys), 1, 1};
-    int e = encode_map(&qmap, type, q, 3, q_sizes, q_strides, q_box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!e) e = encode_map(&kmap, type, pages->k, 4, sizes, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!e) e = encode_map(&vmap, type, pages->v, 4, sizes, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (e) return set_last_error(GPUK_ERR_CUDA, "paged_attention: the driver refused a tensor map (%d)", e);
     int shift = 0;
     while ((1 << shift) < p2) ++shift;
     Joint *joints = static_cast<Joint *>(workspace);
     float *partial = reinterpret_cast<float *>(joints + s.grid);
-    PagedAttentionParams p = {tables, lens, starts, masks, pages->v, out, table_stride, pages->page_stride, pages->head_stride, pages->row_stride, pages->num_pages,
-                              out_token_stride, out_head_stride, batch, tokens, pages->kv_heads, s.group, s.tile_tokens, mask_words, static_cast<uint32_t>(((1ull << 32) + s.tile_tokens - 1) / s.tile_tokens), table_width, shift, s.may_split,
+    PagedAttentionParams p = {tables, lens, starts, masks, q, pages->k, pages->v, out, q_token_stride, q_head_stride, table_stride, pages->page_stride, pages->head_stride, pages->row_stride, pages->num_pages,
+                              out_token_stride, out_head_stride, batch, tokens, pages->kv_heads, s.group, s.tile_tokens, mask_words, static_cast<uint32_t>(((1ull << 32) + s.tile_tokens - 1) / s.tile_tokens), table_width, shift, row_groups_of(s), s.may_split,
                               (reinterpret_cast<uintptr_t>(out) | out_token_stride * 2 | out_head_stride * 2) % 32 == 0,
                               scale * 1.4426950408889634f, d->status, joints, partial, partial + s.grid * 2 * kRows * hd};
     const Kernels k = kernels_of(pages->dtype, hd);
-    void *args[] = {&qmap, &kmap, &vmap, &p};
-    cudaError_t err = launch_kernel(k.attend, static_cast<int>(s.grid), kThreads, 1, false, args, static_cast<cudaStream_t>(stream), k.smem);
+    cudaError_t err;
+    if (single) {
+        int smem = 0;
+        const void *decode = paged_decode_of(pages->dtype, hd, &smem);
+        void *args[] = {&p};
+        err = launch_kernel(decode, static_cast<int>(s.grid), kDecodeThreads, 1, false, args, static_cast<cudaStream_t>(stream), smem);
+    } else {
+        const CUtensorMapDataType type = pages->dtype == GPUK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+        CUtensorMap qmap, kmap, vmap;
+        const uint64_t q_sizes[3] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
+        const uint64_t q_strides[2] = {static_cast<uint64_t>(q_head_stride) * 2, static_cast<uint64_t>(q_token_stride) * 2};
+        const uint32_t q_box[3] = {64, static_cast<uint32_t>(s.group), static_cast<uint32_t>(s.tile_tokens)};
+        const uint64_t sizes[4] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(p2), static_cast<uint64_t>(pages->kv_heads), static_cast<uint64_t>(pages->num_pages)};
+        const uint64_t strides[3] = {static_cast<uint64_t>(pages->row_stride) * 2, static_cast<uint64_t>(pages->head_stride) * 2, static_cast<uint64_t>(pages->page_stride) * 2};
+        const uint32_t box[4] = {64, static_cast<uint32_t>(p2 < kKeys ? p2 : kKeys), 1, 1};
+        int e = encode_map(&qmap, type, q, 3, q_sizes, q_strides, q_box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (!e) e = encode_map(&kmap, type, pages->k, 4, sizes, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (!e) e = encode_map(&vmap, type, pages->v, 4, sizes, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (e) return set_last_error(GPUK_ERR_CUDA, "paged_attention: the driver refused a tensor map (%d)", e);
+        void *args[] = {&qmap, &kmap, &vmap, &p};
+        err = launch_kernel(k.attend, static_cast<int>(s.grid), kThreads, 1, false, args, static_cast<cudaStream_t>(stream), k.smem);
+    }
     if (err == cudaSuccess && s.may_split) {
         void *join_args[] = {&p};
-        err = launch_kernel(k.join, static_cast<int>(s.grid) * kJoinCtas, kJoinWarps * 32, 1, false, join_args, static_cast<cudaStream_t>(stream));
+        err = launch_kernel(k.join, static_cast<int>(s.grid) * p.row_groups, kJoinWarps * 32, 1, false, join_args, static_cast<cudaStream_t>(stream));
     }
     if (err != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_attention: launch failed: %s", cudaGetErrorString(err));
     return GPUK_OK;

@@ -370,9 +370,26 @@ def test_attention_under_masks(ctx, new, words, heads, kv, hd, page, dtype):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("heads,kv,hd,page,dtype", SHAPES[:5])
+@pytest.mark.parametrize("ctx,new", [([300, 20, 1000, 5], [3, 0, 1, 0]), ([0] * 40, [1] * 40), ([5000, 0, 129], [1, 1, 1]), ([31], [1]), ([15, 16, 17, 2049], [0, 2, 0, 2])])
+def test_attention_of_single_tokens(ctx, new, heads, kv, hd, page, dtype):
+    """As many requests as tokens, or more: the kernel for single tokens, and what it does where a request has several or none."""
+    b = _Batch(ctx, new, heads, kv, hd, page, dtype, seed=sum(ctx) + heads)
+    got = b.run()
+    b.check(got)
+    assert torch.equal(got, b.run())
+    for i, (c, n) in enumerate(zip(ctx, new)):      # a value of the last key that is not finite, and a key that is NaN
+        if n:
+            j = c + n - 1
+            b.values[i][j, 0, 3] = math.inf
+            b.v[int(b.tables[i, j // page]), 0, j % page, 3] = math.inf
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("ctx,new", [([70, 500, 3], [2, 40, 9]), ([70, 500, 3] * 17, [1] * 51)])
 @pytest.mark.parametrize("order", ["nhd", "wide"])
-def test_attention_strides(order):
-    b = _Batch([70, 500, 3], [2, 40, 9], 16, 4, 128, 16, order=order)
+def test_attention_strides(order, ctx, new):
+    b = _Batch(ctx, new, 16, 4, 128, 16, order=order)
     got = b.run()
     b.check(got)
     wide = torch.zeros(51, 24, 128, dtype=BF16, device="cuda")
@@ -380,7 +397,7 @@ def test_attention_strides(order):
     out = torch.full((51, 32, 128), 5.0, dtype=BF16, device="cuda")
     again = gpuk.paged_attention(wide[:, 4:20], b.k, b.v, b.tables, b.lens, b.starts, out=out[:, 8:24])
     assert torch.equal(again, got) and bool((out[:, :8] == 5).all()) and bool((out[:, 24:] == 5).all())
-    tables = torch.full((3, 99), -7, dtype=torch.int32, device="cuda")
+    tables = torch.full((len(ctx), 99), -7, dtype=torch.int32, device="cuda")
     tables[:, :b.tables.shape[1]] = b.tables
     assert torch.equal(gpuk.paged_attention(b.q, b.k, b.v, tables[:, :b.tables.shape[1]], b.lens, b.starts), got)
 
