@@ -1,23 +1,31 @@
-// Attention of a ragged batch of new tokens over pages of a KV cache: single tokens, trees of drafted tokens and prompts, heads of 64 and 128, bf16 and fp16.
+// Attention of a ragged batch of new tokens over pages of a KV cache: trees of drafted tokens, prompts and single tokens, heads of 64 and 128, bf16 and fp16.
 //
 // A request has `ctx` cached tokens and `n` new ones, whose keys and values are in its pages already.  A new token sees the cached ones and, of the new ones, those up to
-// itself or those that its bits in `masks` name (in a tree: its ancestors and itself).
+// itself or those that its bits in `masks` name (in a tree: its ancestors and itself).  softmax(scale * q k^T) v, with a running maximum and sum over blocks of 64 keys.
 //
-// One kernel for all of them.  The rows of a tile are pairs of a token and a query head of one kv head's group, tokens outermost: 128 rows are 128 / group tokens, so that a page
-// is read once for a tree of that many nodes, and up to 128 rows cost the tensor pipe less than the page costs HBM (128 operations a byte; the pipe has 250 for each that
-// HBM delivers).  Single tokens leave most rows idle, and warps without a row only keep the barriers going.
+// The rows of a tile are pairs of a token and a query head of one kv head's group, tokens outermost: 128 rows are 128 / group tokens, so that a page is read once for a tree of
+// that many nodes, and up to 128 rows cost the tensor pipe less than the page costs HBM (128 operations a byte; the pipe has 250 for each that HBM delivers).  Calls with no
+// more tokens than requests, whose tiles would be nearly empty, go to paged_decode.cu.
 //
-//   * scores of 64 keys go to one of two buffers in tensor memory, so that the next block's are multiplied while a thread per row works on this one's; the probabilities
-//     go back into the same columns, from where they are the first operand of O += P V.  256 columns and 113 KiB a CTA: two CTAs an SM hide each other's waits.
-//   * pages come by TMA through a ring of 8 or 16 KiB slots; a block of 64 keys is one box of a large page or several small ones, whose numbers the copying warp
-//     reads from the table a block ahead.  Numbers outside the pool and pages behind the last key read as zeros.
-//   * the keys of a tile are cut into parts where the tiles alone do not fill the GPU.  Each CTA works that out from the lengths on the device, the same way, so the host need not
-//     know them; parts leave sums, maxima and outputs in fp32, and a second kernel joins them in order.  The same inputs give the same bits.
+//   * scores go to one of two buffers in tensor memory, so that the next block's are multiplied while a thread per row works on this one's; the probabilities go back into the
+//     same columns, from where they are the first operand of O += P V.  256 columns and 113 KiB a CTA: two CTAs an SM hide each other's waits.
+//   * O is rescaled only where a row's maximum has grown by more than 2^8 (fp16: 2^7) since it was last: otherwise some row of a warp has a new maximum in nearly every block, and each
+//     time 128 columns go through registers (prompts below: 411 us).  The error against float64 is 2.2e-3 in place of 2.0e-3 (1.65e-3 is the result's rounding alone).
+//   * pages come by TMA through a ring of 8 or 16 KiB slots; a block of 64 keys is one box of a large page or several small ones.  The copying warp reads the table 32 boxes at a time, the
+//     next 32 on their way.  Numbers outside the pool and pages behind the last key read as zeros.
+//   * every CTA takes an equal share of all tiles' keys, found from the lengths on the device, so the host need not know them.  A tile that several share leaves sums, maxima and outputs
+//     in fp32, and a second kernel joins them in order: the same inputs give the same bits.
 //   * only blocks that some row sees in part are masked.  There a value that is no finite number would spoil the rows that do not see it (0 * inf), so it is taken out of shared memory
 //     before the product, and the rows that do see it add it at the end.
 //
-// fp32 scores, maxima, sums and outputs.  Probabilities are rounded to the operands' type for the second product; in fp16 they are held times 2^10, so that small
+// fp32 scores, maxima, sums and outputs.  Probabilities are rounded to the operands' type for the second product; in fp16 they are held times 2^8, so that small
 // ones do not fall under its smallest numbers.
+//
+// Measured (64 / 8 heads of 128, pages of 16 and 64): 2 prompts of 2048 behind 0 and 1000 cached tokens, with 4 single tokens, 186 us, 970 TFLOP/s of what the masks leave, 0.58 of the measured
+// bf16 rate; 8 trees of 33 to 64 nodes over 2000 keys 50; 13 nodes over 31 000 keys of 32 / 8 heads of 64, 29.  What bounds it: for prompts the tensor pipe, which takes as long for a product with 64 columns
+// as for one with 128, so that the scores of 64 keys cost as much as their 128 outputs twice over (half the score products left out of a copy: 138 us; the exponentials left out: 169).  Blocks of 128 keys
+// would need 384 columns a CTA, and so one CTA an SM.  For trees and one long context some 9 us of a call are the start of its CTAs, the
+// parts' outputs and the join.  An exponential by polynomial for a quarter of the scores, and two threads a row, did not help: neither unit is the bound.
 #include <cuda_runtime.h>
 
 #include <cmath>
