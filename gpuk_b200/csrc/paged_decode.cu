@@ -11,7 +11,7 @@
 //
 // fp32 scores, running maxima and sums; probabilities are rounded to the operands' type for the second product, in fp16 times 2^8.
 //
-// Measured, 64 / 8 heads of 128, pages of 64: 32 requests of 30 to 4000 keys 39.6 us (194 MB: 4.9 TB/s), of 2049 51.5 (5.2 TB/s), of 300 10.4; 4 of 129 keys, 16 / 4 heads, 5.3.  The tensor-core kernel takes 42.7
+// Measured, 64 / 8 heads of 128, pages of 64: 32 requests of 30 to 4000 keys 39.6 us (194 MB: 4.9 TB/s), of 2049 48.3 (5.6 TB/s), of 300 10.4; 4 of 129 keys, 16 / 4 heads, 5.3.  The tensor-core kernel takes 42.7
 // and 9.7 for the first and 4 x 100 to 300.  Behind HBM stand 5 us for the shares of the CTAs, the cold ring of each of their tiles, and the join.
 #include <cuda_runtime.h>
 

@@ -135,10 +135,11 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
 // One warp for each of a CTA's two borders; lane l looks after a run of the requests.  Quotients are estimated in fp32 and put right, which is faster than dividing 64 bits.
 __device__ void find_border(const PagedAttentionParams &p, Start *out, int side) {
     const int lane = threadIdx.x & 31, per = (p.batch + 31) / 32, lo = min(lane * per, p.batch), hi = min(lo + per, p.batch);
-    int64_t weight = 0, tiles = 0;
+    int64_t weight = 0, tiles = 0, most = 0;
     Request r = {};
     for (int i = lo; i < hi; ++i) {
         r = request_of(p, i);
+        if (r.tiles) most = max(most, weight_of(p, r, r.tiles - 1));
         weight += weight_before(p, r, r.tiles) * p.kv_heads, tiles += static_cast<int64_t>(r.tiles) * p.kv_heads;
     }
     const int64_t upto = warp_scan(weight, lane), all = __shfl_sync(0xffffffffu, upto, 31), before = upto - weight;
@@ -148,6 +149,10 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
     const int border = static_cast<int>(blockIdx.x) + side;
     const int64_t share = static_cast<int64_t>(static_cast<float>(all) * (1.00001f / ctas)) + 1;      // the last CTA's is a little shorter
     const int64_t raw = min(all, border * share);
+    // Tiles are left whole where each has a CTA and none is much more than a share: what parts cost is more than what a more even end gains (single tokens, 32 x 2049 keys of 64 / 8 heads: 48.3 us, 51.5
+    // with cuts; trees of 33 to 64 nodes the same either way).
+    const int64_t largest = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(min(most, static_cast<int64_t>(0x7fffffff))));
+    const bool cut = p.may_split && !(few <= static_cast<int>(gridDim.x) && 2 * largest <= 3 * share);
     if (lane == 0) out->x[side] = all, out->ctas = ctas;      // the line's end, unless a lane below has the border
     __syncwarp();
     if (raw >= all || raw < before || raw >= upto) return;
@@ -173,7 +178,7 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
         }
         const int64_t size = weight_of(p, r, tile);
         int64_t pos = at - first;
-        if (!p.may_split || r.over || pos < kTileCost + kFront) pos = 0;
+        if (!cut || r.over || pos < kTileCost + kFront) pos = 0;
         else if (size - pos < kGrain) pos = size;
         else pos = pos / kKeys * kKeys;      // the borders of blocks, behind the tile's cost
         out->x[side] = base + kvh * head + first + pos;

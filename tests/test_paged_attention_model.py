@@ -177,13 +177,13 @@ def _run(segments, slots, warps, rng, rescales, masked):
     assert not copies and not tensor, "something arrives behind the end"
 
 
-@pytest.mark.parametrize("slots", [4, 9])
+@pytest.mark.parametrize("slots", [5, 10])
 def test_roles_meet(slots):
     rng = random.Random(slots)
     for _ in range(500):
         segments = [rng.choice([1, 1, 2, 3, 4, 5, 9]) for _ in range(rng.choice([1, 2, 3, 6]))]
         often, mask = rng.choice([0.0, 0.2, 1.0]), rng.choice([0.0, 0.3, 1.0])
-        _run(segments, slots, 8, rng, lambda: rng.random() < often, lambda: rng.random() < mask)
+        _run(segments, slots, 4, rng, lambda: rng.random() < often, lambda: rng.random() < mask)
 
 
 # ---- the line of tiles ------------------------------------------------------------------------------------------------
@@ -212,10 +212,14 @@ def _share(requests, kv_heads, tile_tokens, masks, room, grid, may_split=True):
         return min(ctx + (n if masks else min(n, (tile + 1) * tile_tokens)), room)
 
     total = sum(before(r, r[2]) * kv_heads for r in reqs)
-    ctas = min(grid, 2 * sum(r[2] for r in reqs) * kv_heads + total // PER_CTA)
+    few = sum(r[2] for r in reqs) * kv_heads
+    ctas = max(1, min(grid, 2 * few + total // PER_CTA))
+    share = int(total * 1.00001 / ctas) + 1
+    largest = max(before(r, r[2]) - before(r, r[2] - 1) for r in reqs if r[2])
+    may_split = may_split and not (few <= grid and 2 * largest <= 3 * share)
 
     def border(c):
-        raw, base = min(total, c * (int(total * 1.00001 / ctas) + 1)), 0
+        raw, base = min(total, c * share), 0
         for i, r in enumerate(reqs):
             head = before(r, r[2])
             if raw >= base + head * kv_heads:
