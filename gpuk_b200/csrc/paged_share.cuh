@@ -17,6 +17,7 @@ constexpr int kTileCost = 4 * kKeys;             // what a tile costs beside its
 constexpr int kGrain = 2 * kKeys;                // no tile is cut nearer than that to its end, or than kFront to its beginning
 constexpr int kFront = 3 * kKeys;
 constexpr int kPerCta = 256;                     // keys for which a call takes another CTA
+constexpr int kSmall = 6;                        // tiles of a sixth of a CTA's share are not cut
 constexpr float kLowest = -3.4e38f;              // a maximum before any key ...
 constexpr float kSeen = -3.3e38f;                // ... and where all scores are -infinity: finite both, and below any score behind them
 
@@ -149,10 +150,11 @@ __device__ void find_border(const PagedAttentionParams &p, Start *out, int side)
     const int border = static_cast<int>(blockIdx.x) + side;
     const int64_t share = static_cast<int64_t>(static_cast<float>(all) * (1.00001f / ctas)) + 1;      // the last CTA's is a little shorter
     const int64_t raw = min(all, border * share);
-    // Tiles are left whole where each has a CTA and none is much more than a share: what parts cost is more than what a more even end gains (single tokens, 32 x 2049 keys of 64 / 8 heads: 48.3 us, 51.5
-    // with cuts; trees of 33 to 64 nodes the same either way).
+    // Tiles are left whole where each has a CTA and none is much more than a share, and where the largest is a kSmall-th of a share or less: what parts cost is more than what a more even end gains.
+    // 64 / 8 heads, with and without cuts: single tokens of 32 x 2049 keys 51.5 and 48.3 us, of 256 x 2049 372 and 356, 64 trees of 32 behind 2048 223 and 217, 8 prompts of 2048 behind 2048 1586 and 1599.
+    // At a third of a share a prompt of 4096 takes 255 with cuts and 280 without.
     const int64_t largest = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(min(most, static_cast<int64_t>(0x7fffffff))));
-    const bool cut = p.may_split && !(few <= static_cast<int>(gridDim.x) && 2 * largest <= 3 * share);
+    const bool cut = p.may_split && !(few <= static_cast<int>(gridDim.x) && 2 * largest <= 3 * share) && kSmall * largest > share;
     if (lane == 0) out->x[side] = all, out->ctas = ctas;      // the line's end, unless a lane below has the border
     __syncwarp();
     if (raw >= all || raw < before || raw >= upto) return;

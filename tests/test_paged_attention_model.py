@@ -187,7 +187,7 @@ def test_roles_meet(slots):
 
 
 # ---- the line of tiles ------------------------------------------------------------------------------------------------
-KEYS, COST, FRONT, GRAIN, PER_CTA = 64, 256, 192, 128, 256
+KEYS, COST, FRONT, GRAIN, PER_CTA, SMALL = 64, 256, 192, 128, 256, 6
 
 
 def _share(requests, kv_heads, tile_tokens, masks, room, grid, may_split=True):
@@ -216,7 +216,7 @@ def _share(requests, kv_heads, tile_tokens, masks, room, grid, may_split=True):
     ctas = max(1, min(grid, 2 * few + total // PER_CTA))
     share = int(total * 1.00001 / ctas) + 1
     largest = max(before(r, r[2]) - before(r, r[2] - 1) for r in reqs if r[2])
-    may_split = may_split and not (few <= grid and 2 * largest <= 3 * share)
+    may_split = may_split and not (few <= grid and 2 * largest <= 3 * share) and SMALL * largest > share
 
     def border(c):
         raw, base = min(total, c * share), 0
