@@ -46,7 +46,19 @@ const Tensor &heads_arg(PyObject *o, const char *what, int device) {
     dtype_of(t, what);
     return t;
 }
-// The bytes from a tensor's first to its last element.
+// Whether two views with the same strides share an element: whether `distance` is a sum of steps along the dimensions, the longest first, each of which is longer than all shorter ones together.
+struct Step {
+    int64_t stride, least, most;
+};
+bool meet(int64_t distance, const Step *steps, int n) {
+    if (n == 0) return distance == 0;
+    int64_t c = distance / steps->stride;
+    if (c * steps->stride > distance) --c;
+    for (int i = 0; i < 2; ++i, ++c)
+        if (c >= steps->least && c <= steps->most && meet(distance - c * steps->stride, steps + 1, n - 1)) return true;
+    return false;
+}
+// Whether two tensors may share an element: exactly for views of the same strides (heads of one projection's output, keys and values in one allocation), by the bytes that they span for others.
 bool overlap(const Tensor &a, const Tensor &b) {
     if (!a.numel() || !b.numel()) return false;
     auto end = [](const Tensor &t) {
@@ -54,7 +66,25 @@ bool overlap(const Tensor &a, const Tensor &b) {
         for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
         return static_cast<const char *>(t.const_data_ptr()) + (last + 1) * t.element_size();
     };
-    return static_cast<const char *>(a.const_data_ptr()) < end(b) && static_cast<const char *>(b.const_data_ptr()) < end(a);
+    const char *const at = static_cast<const char *>(a.const_data_ptr()), *const bt = static_cast<const char *>(b.const_data_ptr());
+    if (at >= end(b) || bt >= end(a)) return false;
+    const int64_t size = a.element_size();
+    if (a.dim() != b.dim() || a.dim() > 5 || size != static_cast<int64_t>(b.element_size()) || (bt - at) % size) return true;
+    Step steps[5];
+    int n = 0;
+    for (int64_t d = 0; d < a.dim(); ++d) {
+        const int64_t na = a.size(d), nb = b.size(d), stride = na > 1 ? a.stride(d) : b.stride(d);
+        if (na <= 1 && nb <= 1) continue;
+        if (stride <= 0 || (na > 1 && nb > 1 && b.stride(d) != stride)) return true;
+        steps[n++] = {stride, 1 - nb, na - 1};
+    }
+    std::sort(steps, steps + n, [](const Step &x, const Step &y) { return x.stride > y.stride; });
+    int64_t shorter = 0;
+    for (int i = n - 1; i >= 0; --i) {
+        if (shorter >= steps[i].stride) return true;
+        shorter += std::max(steps[i].most, -steps[i].least) * steps[i].stride;
+    }
+    return meet((bt - at) / size, steps, n);
 }
 bool same_place(const Tensor &a, const Tensor &b) { return a.const_data_ptr() == b.const_data_ptr() && a.strides() == b.strides(); }
 
@@ -63,13 +93,17 @@ struct Pages {
     const Tensor &k, &v;
     gpuk_pages c = {};
     int64_t layers = 1, layer_stride = 0;
-    Pages(PyObject *ko, PyObject *vo, int device, bool layered) : k(paged_arg(ko, "k_pages", device)), v(paged_arg(vo, "v_pages", k.get_device())) {
+    Pages(PyObject *ko, PyObject *vo, int device, bool layered, bool written) : k(paged_arg(ko, "k_pages", device)), v(paged_arg(vo, "v_pages", k.get_device())) {
         const int at = layered && k.dim() == 5 ? 1 : 0;
         TORCH_CHECK(k.dim() == 4 + at && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "gpuk: k_pages and v_pages must be [pages, kv_heads, page_size, head_dim], ",
                     "of one size and type");
         c.dtype = dtype_of(k, "k_pages");
         for (int d = 0; d < k.dim(); ++d) TORCH_CHECK(stride_of(k, d) == stride_of(v, d), "gpuk: k_pages and v_pages must have the same strides");
         TORCH_CHECK(k.size(3 + at) <= 1 || k.stride(3 + at) == 1, "gpuk: a token's head must be contiguous in k_pages and v_pages");
+        if (written) {
+            for (int d = 0; d < k.dim(); ++d) TORCH_CHECK(k.size(d) <= 1 || k.stride(d) > 0, "gpuk: k_pages and v_pages repeat their elements");
+            TORCH_CHECK(!overlap(k, v), "gpuk: k_pages and v_pages overlap");
+        }
         if (at) layers = k.size(0), layer_stride = stride_of(k, 0);
         c.k = k.data_ptr(), c.v = v.data_ptr();
         c.page_stride = stride_of(k, at), c.head_stride = stride_of(k, 1 + at), c.row_stride = stride_of(k, 2 + at);
@@ -90,7 +124,10 @@ Tensor heads_out(PyObject *o, const Tensor &like, const char *what) {
     if (o == Py_None) return empty_like_on(like, like.sizes(), like.scalar_type());
     const Tensor &t = heads_arg(o, what, like.get_device());
     TORCH_CHECK(t.sizes() == like.sizes() && t.scalar_type() == like.scalar_type(), "gpuk: ", what, " has another size or type");
-    for (int d = 0; d < 3; ++d) TORCH_CHECK(t.size(d) <= 1 || t.stride(d) > 0, "gpuk: ", what, " repeats its elements");
+    // a token's heads behind one another, or a head's tokens
+    const int64_t n = t.size(2), tokens = t.size(0), heads = t.size(1), token = tokens > 1 ? t.stride(0) : n * heads, head = heads > 1 ? t.stride(1) : n;
+    TORCH_CHECK(!t.numel() || (head >= n && token >= (tokens > 1 ? n : 0) && (heads <= 1 || tokens <= 1 || token >= heads * head || head >= tokens * token)), "gpuk: ", what,
+                " repeats its elements");
     return t;
 }
 
@@ -220,7 +257,7 @@ PyObject *rope_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
     ints_arg(args[5], "frequencies", dev, at::kLong, turns.numel());
     const double amplitude = float_arg(args[6]);
     const int64_t layout = int_arg(args[7]);
-    const Pages pages(args[8], args[9], dev, false);
+    const Pages pages(args[8], args[9], dev, false, true);
     TORCH_CHECK(k.size(0) == tokens && v.sizes() == k.sizes() && k.size(1) == pages.c.kv_heads && k.size(2) == pages.c.head_dim && q.size(2) == pages.c.head_dim,
                 "gpuk: rope_paged shapes do not match");
     TORCH_CHECK(q.scalar_type() == pages.k.scalar_type() && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "gpuk: rope_paged takes one type");
@@ -231,7 +268,7 @@ PyObject *rope_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
         out = heads_out(args[10], q, "out");
         TORCH_CHECK((!overlap(out, q) || (same_place(out, q) && layout != GPUK_ROPE_SPLIT)), "gpuk: rope_paged: out overlaps q");
         for (const Tensor *t : std::initializer_list<const Tensor *>{&out, &q, &k, &v}) TORCH_CHECK(!overlap(*t, pages.k) && !overlap(*t, pages.v), "gpuk: rope_paged: a tensor overlaps the pages");
-        if (!same_place(out, q)) TORCH_CHECK(!overlap(out, k) && !overlap(out, v), "gpuk: rope_paged: out overlaps k or v");
+        TORCH_CHECK(!overlap(out, k) && !overlap(out, v), "gpuk: rope_paged: out overlaps k or v");
         check(gpuk_rope_paged(q.const_data_ptr(), stride_of(q, 0), stride_of(q, 1), k.const_data_ptr(), stride_of(k, 0), stride_of(k, 1), v.const_data_ptr(), stride_of(v, 0),
                               stride_of(v, 1), out.data_ptr(), stride_of(out, 0), stride_of(out, 1), pos.data_ptr<int64_t>(), slots.data_ptr<int64_t>(), turns.data_ptr<int64_t>(),
                               static_cast<float>(amplitude), &pages.c, int_size(tokens), int_size(q.size(1)), int_size(2 * turns.numel()), int_size(layout), stream_of(q)),
@@ -247,7 +284,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     expect_args(n, 10, "paged_attention");
     const Tensor &q = heads_arg(args[0], "q", -1);
     const int dev = q.get_device();
-    const Pages pages(args[1], args[2], dev, false);
+    const Pages pages(args[1], args[2], dev, false, false);
     const Tensor &lens = paged_arg(args[4], "lens", dev);
     TORCH_CHECK(lens.dim() == 1, "gpuk: lens must be one-dimensional");
     const int64_t batch = lens.size(0), tokens = q.size(0);
@@ -288,7 +325,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *paged_keep(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect_args(n, 6, "paged_keep");
-    const Pages pages(args[0], args[1], -1, true);
+    const Pages pages(args[0], args[1], -1, true, true);
     const int dev = pages.k.get_device();
     const Tensor &lens = paged_arg(args[3], "lens", dev);
     TORCH_CHECK(lens.dim() == 1, "gpuk: lens must be one-dimensional");
@@ -300,7 +337,6 @@ PyObject *paged_keep(PyObject *, PyObject *const *args, Py_ssize_t n) {
         out = ints_arg(args[5], "out", dev, at::kInt, batch);
         for (const Tensor *t : std::initializer_list<const Tensor *>{&lens, &tables, &paths}) TORCH_CHECK(!overlap(out, *t), "gpuk: paged_keep: out overlaps what is read");
     }
-    TORCH_CHECK(!overlap(pages.k, pages.v), "gpuk: paged_keep: k_pages and v_pages overlap");
     {
         NoGil unlocked;
         c10::cuda::CUDAGuard guard(pages.k.device());

@@ -134,7 +134,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, paths: torch.Tensor, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Makes the accepted path of each request's tree its next cached tokens: new token ``paths[i, j]`` moves to ``lens[i] + j``, in ``k_pages`` and ``v_pages`` of one layer or
-    [layers, pages, kv_heads, page_size, head_dim] of all.  A path ascends and ends at its first entry that does not (-1).  Returns the new lengths."""
+    [layers, pages, kv_heads, page_size, head_dim] of all.  A path ascends and ends at its first entry that does not (-1); it names
+    tokens of the last plan only, for only they have pages.  Returns the new lengths."""
     return _native.paged_keep(k_pages, v_pages, tables, lens, paths, out)
 
 

@@ -539,3 +539,49 @@ def test_keep_at_the_table_s_end():
     want[1, :, 2] = k[1, :, 3]
     got = gpuk.paged_keep(k, v, _ints([[1, -1], [0, 5]]), _ints([2, 7]), _ints([[1, 9, 400], [1, 2, 3]]))
     assert got.tolist() == [5, 10] and torch.equal(k, want) and torch.equal(v, want)
+
+
+# ---- views of one allocation -----------------------------------------------------------------------------
+@pytest.mark.parametrize("order", ["pages", "rows", "layers"])
+def test_keys_and_values_of_one_allocation(order):
+    """Keys and values as the two halves of each page, of each row, or of the whole pool: the same bits as in pools of their own."""
+    pages, kv, page, hd, n = 9, 2, 16, 64, 40
+    both = torch.zeros({"pages": (pages, 2, kv, page, hd), "rows": (pages, kv, page, 2, hd), "layers": (2, pages, kv, page, hd)}[order], dtype=BF16, device="cuda")
+    k, v = both.unbind({"pages": 1, "rows": 3, "layers": 0}[order])
+    own_k, own_v = torch.zeros_like(k, memory_format=torch.contiguous_format), torch.zeros_like(k, memory_format=torch.contiguous_format)
+    g = torch.Generator().manual_seed(5)
+    x, q = torch.randn(2, n, kv, hd, generator=g).to(BF16).cuda(), torch.randn(n, 6, hd, generator=g).to(BF16).cuda()
+    tables, lens, f = _ints([[7, 2, 4, -1]]), _ints([0]), gpuk.rope_frequencies(hd, device="cuda")
+    at = torch.arange(n, device="cuda")
+    slots = tables[0].long()[at // page] * page + at % page
+    got = []
+    for kc, vc in ((k, v), (own_k, own_v)):
+        rotated = gpuk.rope_paged(q, x[0], x[1], at, slots, f, kc, vc)
+        out = [rotated] + [gpuk.paged_attention(rotated[a:], kc, vc, tables, _ints([a]), _ints([0, n - a])) for a in (0, n - 1)]
+        got.append(out + [gpuk.paged_keep(kc, vc, tables, lens, _ints([[1, 5, 30]])), kc.clone(), vc.clone()])
+    _status_ok()
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and bool(got[0][-1].any())
+
+
+def test_queries_in_place_beside_their_keys():
+    """Queries of a joint projection are rotated where they are; what would be read behind a write, or written twice, is refused."""
+    x = torch.randn(5, 12, 64, generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    at, f = torch.arange(5, device="cuda"), gpuk.rope_frequencies(64, device="cuda")
+    k, v = _pool(1, 4, 8, 64, BF16), _pool(1, 4, 8, 64, BF16)
+    parts = [x.split([4, 4, 4], dim=1), x.view(5, 4, 3, 64).unbind(2)]      # heads one after another, and each with its key and value
+    for i in range(2):
+        want = gpuk.rope_paged(*parts[i], at, at, f, k, v)
+        held, before = (k.clone(), v.clone()), x.clone()
+        q = parts[i][0]
+        assert torch.equal(gpuk.rope_paged(*parts[i], at, at, f, k, v, out=q), want) and torch.equal(q, want)
+        assert torch.equal(k, held[0]) and torch.equal(v, held[1])
+        q.copy_((before.split([4, 4, 4], dim=1)[0] if i == 0 else before.view(5, 4, 3, 64)[:, :, 0]))
+        assert torch.equal(x, before)
+    q, kx, vx = parts[0]
+    twice = torch.zeros(400, dtype=BF16, device="cuda").as_strided((5, 4, 64), (64, 8, 1))
+    for call, text in [(lambda: gpuk.rope_paged(q, q, vx, at, at, f, k, v, out=q), "overlaps k or v"), (lambda: gpuk.rope_paged(q, x[:, 3:7], vx, at, at, f, k, v, out=q), "overlaps k or v"),
+                       (lambda: gpuk.rope_paged(q, kx, vx, at, at, f, k, k), "overlap"), (lambda: gpuk.rope_paged(q, kx, vx, at, at, f, k[:, :, :1].expand(1, 4, 8, 64), v[:, :, :1].expand(1, 4, 8, 64)), "repeat"),
+                       (lambda: gpuk.rope(q, at, f, out=twice), "repeats"), (lambda: gpuk.rope(q, at, f, out=twice[:1].expand(5, 4, 64)), "repeats")]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+    torch.cuda.synchronize()
