@@ -24,7 +24,7 @@
 // Measured (64 / 8 heads of 128, pages of 16 and 64): 2 prompts of 2048 behind 0 and 1000 cached tokens, with 4 single tokens, 186 us, 970 TFLOP/s of what the masks leave, 0.58 of the measured
 // bf16 rate; 8 trees of 33 to 64 nodes over 2000 keys 50; 13 nodes over 31 000 keys of 32 / 8 heads of 64, 29.  What bounds it: for prompts the tensor pipe, which takes as long for a product with 64 columns
 // as for one with 128, so that the scores of 64 keys cost as much as their 128 outputs twice over (half the score products left out of a copy: 138 us; the exponentials left out: 169).  Blocks of 128 keys
-// would need 384 columns a CTA, and so one CTA an SM.  For trees and one long context some 9 us of a call are the start of its CTAs, the
+// with two score buffers would need 384 columns a CTA, and so one CTA an SM; with one buffer nothing is multiplied while the rows work on it, and the prompts take 220.  For trees and one long context some 9 us of a call are the start of its CTAs, the
 // parts' outputs and the join.  An exponential by polynomial for a quarter of the scores, and two threads a row, did not help: neither unit is the bound.
 #include <cuda_runtime.h>
 
