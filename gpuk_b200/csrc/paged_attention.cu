@@ -24,8 +24,9 @@
 // Measured (64 / 8 heads of 128, pages of 16 and 64): 2 prompts of 2048 behind 0 and 1000 cached tokens, with 4 single tokens, 186 us, 970 TFLOP/s of what the masks leave, 0.58 of the measured
 // bf16 rate; 8 trees of 33 to 64 nodes over 2000 keys 50; 13 nodes over 31 000 keys of 32 / 8 heads of 64, 29.  What bounds it: for prompts the tensor pipe, which takes as long for a product with 64 columns
 // as for one with 128, so that the scores of 64 keys cost as much as their 128 outputs twice over (half the score products left out of a copy: 138 us; the exponentials left out: 169).  Blocks of 128 keys
-// with two score buffers would need 384 columns a CTA, and so one CTA an SM; with one buffer nothing is multiplied while the rows work on it, and the prompts take 220.  For trees and one long context some 9 us of a call are the start of its CTAs, the
-// parts' outputs and the join.  An exponential by polynomial for a quarter of the scores, and two threads a row, did not help: neither unit is the bound.
+// with two score buffers would need 384 columns a CTA, and so one CTA an SM; with one buffer nothing is multiplied while the rows work on it, and the prompts take 220; one CTA an SM with three
+// buffers, whose row threads take the blocks in turn with a second 128, takes 320 (long prompts 1.2 times as long), since nothing hides a tile's start and end.  For trees and one long context some
+// 9 us of a call are the start of its CTAs, the parts' outputs and the join.  An exponential by polynomial for a quarter of the scores, and two threads a row, did not help: neither unit is the bound.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -59,7 +60,7 @@ template <int HD>
 struct Smem {
     alignas(1024) unsigned char q[HD / 64 * kQSpanBytes];
     alignas(1024) unsigned char ring[kSlotsOf<HD>][HD / 64 * kSpanBytes];
-    uint64_t q_full[2], q_empty, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done[2], drained;
+    uint64_t q_full[2], q_empty, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done[2], together, drained;
     Segment queue[kQueue];
     Start start;
     uint32_t tmem;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     if (tid == kRows) {
         for (int b = 0; b < 2; ++b) mbar_init(&sm.q_full[b], 1), mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows / 32), mbar_init(&sm.o_done[b], 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-        mbar_init(&sm.q_empty, 1), mbar_init(&sm.drained, 1);
+        mbar_init(&sm.q_empty, 1), mbar_init(&sm.together, kRows / 32), mbar_init(&sm.drained, 1);
         mbar_init_fence();
     }
     if (tid >= kRows + 32)
@@ -432,7 +433,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             fill += 2 * u.blocks;
             if (ok) ok = wait_at(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
             tc_fence_after();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            // all rows' warps have come here, or one of them has given up: a named barrier would wait for it without end
+            __syncwarp();
+            if ((tid & 31) == 0) arrive_at(smem_addr(&sm.together));
+            if (ok) ok = wait_at(smem_addr(&sm.together), segment & 1);
             if (busy) {
                 uint32_t any = 0;
 #pragma unroll

@@ -33,7 +33,7 @@ def _wait(barrier, index):
 def _run(segments, slots, warps, rng, rescales, masked):
     full, empty = [Barrier(1) for _ in range(slots)], [Barrier(1) for _ in range(slots)]
     q_full, s_full, o_done, p_full = ([Barrier(n) for _ in range(2)] for n in (1, 1, 1, warps))
-    q_empty = Barrier(1)
+    q_empty, together = Barrier(1), Barrier(warps)
     queue, copies, tensor = [None] * QUEUE, [], []
     q_held, ring, scores_done, product_done = [None], [None] * slots, [-1], [-1]
     reading_ring, reading_queue = [0] * slots, [0] * QUEUE
@@ -133,6 +133,8 @@ def _run(segments, slots, warps, rng, rescales, masked):
             fill += 2 * blocks
             yield from _wait(o_done[(t - 1) & 1], (t - 1) >> 1)
             assert product_done[0] == t - 1
+            together.arrive()
+            yield from _wait(together, number)
             yield True
             assert product_done[0] == t - 1      # the outputs stay while they are read
             number += 1
