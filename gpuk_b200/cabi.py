@@ -97,7 +97,7 @@ _SIGNATURES = {
     "gpuk_rope": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, c_float] + [c_int] * 6 + [_P]),
     "gpuk_rope_paged": (c_int, [_P, c_int64, c_int64] * 4 + [_P, _P, _P, c_float, POINTER(Pages)] + [c_int] * 4 + [_P]),
     "gpuk_paged_attention_workspace": (c_int, [POINTER(Pages), c_int, c_int, c_int, c_int64, POINTER(c_int64)]),
-    "gpuk_paged_attention": (c_int, [_P, c_int64, c_int64, POINTER(Pages), _P, c_int64, c_int, _P, _P, _P, c_int, _P, c_int64, c_int64, c_int, c_int, c_int, c_int64,
+    "gpuk_paged_attention": (c_int, [_P, c_int64, c_int64, POINTER(Pages), _P, c_int64, c_int, _P, _P, _P, c_int, _P, c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int,
                                      c_float, _P, c_int64, _P]),
     "gpuk_paged_keep": (c_int, [POINTER(Pages), c_int, c_int64, _P, c_int64, c_int, _P, _P, c_int64, c_int, _P, c_int, _P]),
 }

@@ -278,10 +278,11 @@ PyObject *rope_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// paged_attention(q [tokens, heads, head_dim], k_pages, v_pages, tables, lens, starts, masks or None, max_len (negative: what the table holds), scale (0: 1 / sqrt(head_dim)), out or None)
+// paged_attention(q [tokens, heads, head_dim], k_pages, v_pages, tables, lens, starts, masks or None, max_len (negative: what the table holds), max_new (0: not known),
+// scale (0: 1 / sqrt(head_dim)), out or None)
 PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect_args(n, 10, "paged_attention");
+    expect_args(n, 11, "paged_attention");
     const Tensor &q = heads_arg(args[0], "q", -1);
     const int dev = q.get_device();
     const Pages pages(args[1], args[2], dev, false, false);
@@ -296,7 +297,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         TORCH_CHECK(masks->is_contiguous() && masks->size(1) >= 1, "gpuk: masks must be contiguous, with a word or more");
     }
     int64_t max_len = int_arg(args[7]);
-    double scale = float_arg(args[8]);
+    const int max_new = int_size(int_arg(args[8]));
+    double scale = float_arg(args[9]);
     TORCH_CHECK(q.size(2) == pages.c.head_dim && q.scalar_type() == pages.k.scalar_type(), "gpuk: paged_attention: q and the pages have different heads or types");
     if (scale == 0.0) scale = 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(1, q.size(2))));
     const int64_t holds = tables.size(1) * pages.c.page_size;
@@ -305,7 +307,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     {
         NoGil unlocked;
         c10::cuda::CUDAGuard guard(q.device());
-        out = heads_out(args[9], q, "out");
+        out = heads_out(args[10], q, "out");
         TORCH_CHECK(!overlap(out, q) && !overlap(out, pages.k) && !overlap(out, pages.v), "gpuk: paged_attention: out overlaps what is read");
         int64_t bytes = 0;
         check(gpuk_paged_attention_workspace(&pages.c, int_size(batch), int_size(tokens), int_size(q.size(1)), max_len, &bytes), "paged_attention");
@@ -314,7 +316,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (bytes) workspace = empty_like_on(q, {bytes}, at::kByte);
         check(gpuk_paged_attention(q.const_data_ptr(), stride_of(q, 0), stride_of(q, 1), &pages.c, tables.data_ptr<int>(), batch > 1 ? tables.stride(0) : tables.size(1),
                                    int_size(tables.size(1)), lens.data_ptr<int>(), starts.data_ptr<int>(), masks ? masks->data_ptr<int>() : nullptr, masks ? int_size(masks->size(1)) : 0,
-                                   out.data_ptr(), stride_of(out, 0), stride_of(out, 1), int_size(batch), int_size(tokens), int_size(q.size(1)), max_len, static_cast<float>(scale),
+                                   out.data_ptr(), stride_of(out, 0), stride_of(out, 1), int_size(batch), int_size(tokens), int_size(q.size(1)), max_len, max_new, static_cast<float>(scale),
                                    bytes ? workspace.data_ptr() : nullptr, bytes, stream_of(q)), "paged_attention");
     }
     return THPVariable_Wrap(std::move(out));

@@ -586,8 +586,9 @@ struct Shape {
     int group, tile_tokens, may_split;
     int64_t grid, bytes;
 };
-// `single`: no more new tokens than requests, and so in all likelihood one for each.  Both kernels give the formula's result whatever the requests have; for single tokens the one that is built
-// for them takes 4 x 100 to 300 keys of 16 / 4 heads in 6.6 us instead of 9.7, 32 x 30 to 4000 of 64 / 8 in 39.4 instead of 42.7.
+// `single`: single tokens, or without a bound on a request's new ones no more of them than requests, and so in all likelihood one for each.  Both kernels give the formula's result whatever the
+// requests have; for single tokens the one that is built for them takes 4 x 100 to 300 keys of 16 / 4 heads in 6.6 us instead of 9.7, 32 x 30 to 4000 of 64 / 8 in 39.4 instead of 42.7.  For many tokens of a few of the
+// requests it is the other way round: 64 of one behind 2000 keys 64 us, 23 by the tensor-core kernel; 8 behind nothing 4.8 and 6.9.
 Shape shape_of(int batch, int tokens, int heads, int kv_heads, int head_dim, int64_t max_len, int sms, bool single) {
     Shape s = {};
     s.group = heads / kv_heads;
@@ -603,7 +604,9 @@ Shape shape_of(int batch, int tokens, int heads, int kv_heads, int head_dim, int
 }
 
 int row_groups_of(const Shape &s) { return (s.tile_tokens * s.group + 31) / 32; }
-bool single_tokens(int batch, int tokens, int heads, int kv_heads, bool masks) { return !masks && tokens <= batch && heads / kv_heads <= kDecodeGroup; }
+bool single_tokens(int batch, int tokens, int max_new, int heads, int kv_heads, bool masks) {
+    return !masks && (max_new ? max_new == 1 : tokens <= batch) && heads / kv_heads <= kDecodeGroup;
+}
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_shape(const gpuk_pages *pages, int batch, int tokens, int heads, int64_t max_len) {
@@ -645,9 +648,9 @@ extern "C" int gpuk_paged_attention_workspace(const gpuk_pages *pages, int batch
     const DecodeDevice *d = nullptr;
     rc = decode_device(&d);
     if (rc != GPUK_OK) return rc;
-    // of the kernel that needs more: which one a call takes depends on its masks too
+    // of the kernel that needs more: which one a call takes depends on its masks and on max_new too
     for (bool single : {false, true}) {
-        if (single && !single_tokens(batch, tokens, heads, pages->kv_heads, false)) continue;
+        if (single && !single_tokens(batch, tokens, 1, heads, pages->kv_heads, false)) continue;
         const int64_t need = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms, single).bytes;
         if (need > *bytes) *bytes = need;
     }
@@ -656,10 +659,10 @@ extern "C" int gpuk_paged_attention_workspace(const gpuk_pages *pages, int batch
 
 extern "C" int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const gpuk_pages *pages, const int32_t *tables, int64_t table_stride, int table_width,
                                     const int32_t *lens, const int32_t *starts, const int32_t *masks, int mask_words, void *out, int64_t out_token_stride, int64_t out_head_stride,
-                                    int batch, int tokens, int heads, int64_t max_len, float scale, void *workspace, int64_t workspace_bytes, void *stream) {
+                                    int batch, int tokens, int heads, int64_t max_len, int max_new, float scale, void *workspace, int64_t workspace_bytes, void *stream) {
     int rc = check_shape(pages, batch, tokens, heads, max_len);
     if (rc != GPUK_OK) return rc;
-    if (table_width < 0 || mask_words < 0 || (masks && mask_words == 0)) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: bad sizes");
+    if (table_width < 0 || mask_words < 0 || max_new < 0 || (masks && mask_words == 0)) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: bad sizes");
     if (!(scale > 0.f) || std::isinf(scale)) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_attention: the scale must be a positive number");
     const int p2 = pages->page_size;
     if (p2 < 8 || (p2 & (p2 - 1)) || p2 > 65536) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: pages of %d tokens; built for powers of two from 8 to 65536", p2);
@@ -676,7 +679,7 @@ extern "C" int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64
     const DecodeDevice *d = nullptr;
     rc = decode_device(&d);
     if (rc != GPUK_OK) return rc;
-    const bool single = single_tokens(batch, tokens, heads, pages->kv_heads, masks != nullptr);
+    const bool single = single_tokens(batch, tokens, max_new, heads, pages->kv_heads, masks != nullptr);
     const Shape s = shape_of(batch, tokens, heads, pages->kv_heads, pages->head_dim, max_len, d->sms, single);
     if (s.grid * row_groups_of(s) > 0x7fffffffll) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_attention: too many tokens");
     if (s.may_split && (!workspace || workspace_bytes < s.bytes || !aligned16(workspace)))

@@ -120,16 +120,21 @@ def rope_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, *,
-                    masks: Optional[torch.Tensor] = None, max_len: Optional[int] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    masks: Optional[torch.Tensor] = None, max_len: Optional[int] = None, max_new: Optional[int] = None, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the new tokens ``q`` [tokens, heads, head_dim] over their requests' pages, in which their own keys and values are already, behind ``lens`` cached ones.
 
     A token sees the cached ones and, of its request's new ones, those up to itself, or with ``masks`` (``PagedPlan.masks``, or any words [tokens, words <= 8]) those whose bits are
     set.  One that sees no key gets zeros; what it does not see does not reach it, be it infinite or NaN.  Rows behind ``starts[-1]`` are left as they are in
-    ``out``.  ``max_len`` bounds cached plus new tokens of a request (default: what the table holds): a speed hint.  ``scale`` defaults to 1 / sqrt(head_dim).  Heads
-    of 64 or 128, bf16 or fp16, pages of 8 tokens or more; the same inputs give the same bits."""
+    ``out``.  ``max_len`` bounds cached plus new tokens of a request (default: what the table holds), ``max_new`` the new tokens of
+    one (default: 1 in calls with no more tokens than requests): speed hints, which change no more than the order of sums.  ``scale`` defaults to
+    1 / sqrt(head_dim).  Heads of 64 or 128, bf16 or fp16, pages of 8 tokens or more; the same inputs give the same bits."""
     if scale is not None and not 0.0 < scale < math.inf:
         raise ValueError(f"gpuk: a scale of {scale} is no positive number")
-    return _native.paged_attention(q, k_pages, v_pages, tables, lens, starts, masks, -1 if max_len is None else max_len, 0.0 if scale is None else scale, out)
+    if max_new is not None and max_new < 1:
+        raise ValueError(f"gpuk: at most {max_new} new tokens of a request")
+    return _native.paged_attention(q, k_pages, v_pages, tables, lens, starts, masks, -1 if max_len is None else max_len, 0 if max_new is None else max_new,
+                                   0.0 if scale is None else scale, out)
 
 
 def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, paths: torch.Tensor, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:

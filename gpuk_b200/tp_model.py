@@ -335,11 +335,13 @@ class TPDecoder:
         return gpuk.PagedKVCache(a.n_layers, pages, page_size, self.kv_local, a.head_dim, requests, pages_per_request, dtype=a.dtype, device=self.device)
 
     @torch.no_grad()
-    def forward_paged(self, tokens: torch.Tensor, cache: gpuk.PagedKVCache, plan: gpuk.PagedPlan, max_len: Optional[int] = None) -> torch.Tensor:
+    def forward_paged(self, tokens: torch.Tensor, cache: gpuk.PagedKVCache, plan: gpuk.PagedPlan, max_len: Optional[int] = None,
+                      max_new: Optional[int] = None) -> torch.Tensor:
         """tokens [total], the new ones of all requests one after another as ``plan`` (``cache.plan``) has them -> logits [total, vocab/world] of this rank's vocabulary
         shard.  Requests may be of any lengths and have any number of new tokens: one each, a tree of drafts to be verified, a prompt.  Their keys and values are in the
         cache's pages afterwards, and count from ``cache.append`` or ``cache.keep`` on.  Logits of a token without a slot are NaN; those of rows behind the last request
-        mean nothing.  ``max_len``: no request has more cached and new tokens.  Heads of 64 or 128; there is no CPU path."""
+        mean nothing.  ``max_len``: no request has more cached and new tokens; ``max_new``: none has more new ones
+        (worth to say where a few of many requests have some: ``paged_attention``).  Heads of 64 or 128; there is no CPU path."""
         a = self.args
         if self.device.type != "cuda":
             raise RuntimeError("gpuk: a paged cache needs a CUDA device")
@@ -354,6 +356,6 @@ class TPDecoder:
             k_pages, v_pages = cache.k[li], cache.v[li]
             q, k, v = layer["wqkv"](normed, scale).view(-1, sum(heads), hd).split(heads, dim=1)
             q = gpuk.rope_paged(q, k, v, plan.positions, plan.slots, self.frequencies, k_pages, v_pages, layout="split")
-            att = gpuk.paged_attention(q, k_pages, v_pages, cache.tables, cache.lens, plan.starts, masks=plan.masks, max_len=max_len)
+            att = gpuk.paged_attention(q, k_pages, v_pages, cache.tables, cache.lens, plan.starts, masks=plan.masks, max_len=max_len, max_new=max_new)
             h, normed, scale = self._after_attention(li, att.view(-1, self.h_local * hd), h, self.own_elementwise)
         return self.output(normed, scale)

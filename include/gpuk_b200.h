@@ -457,13 +457,13 @@ int gpuk_rope_paged(const void *q, int64_t q_token_stride, int64_t q_head_stride
  * behind lens[i] cached tokens.  A new token sees all cached ones and, of the new ones, those up to itself, or with masks [tokens, mask_words] those whose bit is set
  * (bit j: new token j of its request).  A row that sees no key is zeros; keys that a row does not see do not reach it, be they infinite or NaN.  Rows of q
  * behind starts[batch] are not read and those of out not written.  Heads of 64 and 128, up to 128 query heads per kv head, bf16 and fp16, pages of at least 8 tokens.  Pages outside
- * the pool read as zeros.  max_len: no request has more cached and new tokens (it decides whether keys are split over CTAs, not the result).  q and out: strides
- * in values, positive multiples of 8, 16-byte aligned.  The workspace belongs to the call until it is done on the stream.
+ * the pool read as zeros.  max_len: no request has more cached and new tokens (it decides whether keys are split over CTAs, not the result).  max_new:
+ * no request has more new tokens, 0 if that is not known (it decides between a kernel for single tokens and one for many, not the result).  q and out: strides in values, positive multiples of 8, 16-byte aligned.  The workspace belongs to the call until it is done on the stream.
  */
 int gpuk_paged_attention_workspace(const gpuk_pages *pages, int batch, int tokens, int heads, int64_t max_len, int64_t *bytes);
 int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const gpuk_pages *pages, const int32_t *tables, int64_t table_stride, int table_width,
                          const int32_t *lens, const int32_t *starts, const int32_t *masks, int mask_words, void *out, int64_t out_token_stride, int64_t out_head_stride,
-                         int batch, int tokens, int heads, int64_t max_len, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+                         int batch, int tokens, int heads, int64_t max_len, int max_new, float scale, void *workspace, int64_t workspace_bytes, void *stream);
 /*
  * The accepted path of each request's tree: new token path[j] becomes cached token lens + j, in `layers` layers of keys and values.  A path [depth] ascends
  * strictly from 0 or more and ends at the first entry that does not (-1 by habit).  lens_out[i] = lens[i] + its length; lens_out is not lens.

@@ -460,6 +460,23 @@ def test_the_bound_on_lengths_is_a_hint():
         b.check(b.run(max_len=bound))
 
 
+@pytest.mark.parametrize("heads,kv,hd,page,dtype", SHAPES)
+def test_the_bound_on_new_tokens_is_a_hint(heads, kv, hd, page, dtype):
+    """Either kernel, with few and many requests, where the bound is true, too large or too small."""
+    for ctx, new in [([500] + [0] * 30, [20] + [0] * 30), ([70, 3, 900, 0], [1, 1, 1, 1]), ([64, 300], [5, 130])]:
+        b = _Batch(ctx, new, heads, kv, hd, page, dtype)
+        for bound in (1, 2, max(new), 1 << 20):
+            b.check(b.run(max_new=bound))
+        # rows behind the last request, more of them than requests
+        padded = torch.cat([b.q, b.q[:1].expand(len(new) + 3, -1, -1)])
+        out = torch.full_like(padded, 3.0)
+        gpuk.paged_attention(padded, b.k, b.v, b.tables, b.lens, b.starts, max_new=1, out=out)
+        b.check(out[:sum(new)])
+        assert bool((out[sum(new):] == 3).all())
+    with pytest.raises(ValueError, match="new tokens"):
+        b.run(max_new=0)
+
+
 def test_more_tokens_than_the_table_holds():
     """Those behind the row's end have no keys: they see what there is; nothing is read outside the row."""
     b = _Batch([16], [40], 4, 2, 64, 16, spare=9)

@@ -36,7 +36,7 @@ def test_plan_refusals(more, status, text):
 
 def _attention(pages=None, **more):
     v = dict(q=P, qt=256, qh=64, pages=pages or _pages(), tables=P, stride=4, width=4, lens=P, starts=P, masks=None, words=0, out=P, ot=256, oh=64, batch=2, tokens=8, heads=4,
-             max_len=64, scale=0.125, ws=None, bytes=0)
+             max_len=64, max_new=0, scale=0.125, ws=None, bytes=0)
     v.update(more)
     return cabi.lib.gpuk_paged_attention(*v.values(), None)
 
@@ -47,7 +47,7 @@ def _attention(pages=None, **more):
     ({"pages": _pages(page_size=4)}, cabi.ERR_UNSUPPORTED, "powers of two"), ({"pages": _pages(page_size=48)}, cabi.ERR_UNSUPPORTED, "powers of two"),
     ({"masks": P, "words": 9}, cabi.ERR_UNSUPPORTED, "8"), ({"masks": P}, cabi.ERR_INVALID_ARGUMENT, "sizes"), ({"scale": 0.0}, cabi.ERR_INVALID_ARGUMENT, "scale"),
     ({"scale": -1.0}, cabi.ERR_INVALID_ARGUMENT, "scale"), ({"scale": float("nan")}, cabi.ERR_INVALID_ARGUMENT, "scale"), ({"scale": float("inf")}, cabi.ERR_INVALID_ARGUMENT, "scale"),
-    ({"tokens": (1 << 24) + 1}, cabi.ERR_UNSUPPORTED, "2\\^24"), ({"tokens": -1}, cabi.ERR_INVALID_ARGUMENT, "sizes"), ({"q": None}, cabi.ERR_INVALID_ARGUMENT, "null"),
+    ({"tokens": (1 << 24) + 1}, cabi.ERR_UNSUPPORTED, "2\\^24"), ({"tokens": -1}, cabi.ERR_INVALID_ARGUMENT, "sizes"), ({"max_new": -1}, cabi.ERR_INVALID_ARGUMENT, "sizes"), ({"q": None}, cabi.ERR_INVALID_ARGUMENT, "null"),
     ({"tables": None}, cabi.ERR_INVALID_ARGUMENT, "null"), ({"pages": _pages(num_pages=0)}, cabi.ERR_INVALID_ARGUMENT, "no pages"), ({"width": 0}, cabi.ERR_INVALID_ARGUMENT, "no pages"),
     ({"q": P + 8}, cabi.ERR_INVALID_ARGUMENT, "aligned"), ({"pages": _pages(v=P + 2)}, cabi.ERR_INVALID_ARGUMENT, "aligned"), ({"qt": 12}, cabi.ERR_INVALID_ARGUMENT, "strides"),
     ({"qh": 0}, cabi.ERR_INVALID_ARGUMENT, "strides"), ({"pages": _pages(row_stride=68)}, cabi.ERR_INVALID_ARGUMENT, "strides"), ({"width": 1 << 28}, cabi.ERR_UNSUPPORTED, "too wide")])
