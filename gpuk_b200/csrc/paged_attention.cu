@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             const int tok = u.tok0 + row_tok;
             const bool valid = tid < p.tile_tokens * p.group && tok < u.n;
             const bool busy = __any_sync(0xffffffffu, valid);
-            // blocks from here on hold keys that some row does not see, or none
-            const int64_t limit = p.masks ? u.ctx : static_cast<int64_t>(u.ctx) + u.tok0 + 1;
+            // blocks from here on hold keys that some row does not see, or none: a tile may begin behind the end of the table's row, inside whose last block the keys end
+            const int64_t limit = p.masks ? u.ctx : min(static_cast<int64_t>(u.ctx) + u.tok0 + 1, room_of(p));
             const int first_masked = max(u.first, static_cast<int>(limit / kKeys));
             uint32_t *poison = sm.poison[segment % 3];
             if (tid < kMaskedBlocks * 2) sm.poison[(segment + 1) % 3][tid] = 0;      // read last before the barrier of the segment in front
