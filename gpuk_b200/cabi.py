@@ -100,6 +100,7 @@ _SIGNATURES = {
     "gpuk_paged_attention": (c_int, [_P, c_int64, c_int64, POINTER(Pages), _P, c_int64, c_int, _P, _P, _P, c_int, _P, c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int,
                                      c_float, _P, c_int64, _P]),
     "gpuk_paged_keep": (c_int, [POINTER(Pages), c_int, c_int64, _P, c_int64, c_int, _P, _P, c_int64, c_int, _P, c_int, _P]),
+    "gpuk_paged_keep_held": (c_int, [POINTER(Pages), c_int, c_int64, _P, c_int64, c_int, _P, _P, c_int64, c_int, _P, _P, c_int, _P]),
 }
 for _name, (_res, _args) in _SIGNATURES.items():
     _fn = getattr(lib, _name)

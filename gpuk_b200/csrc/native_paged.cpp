@@ -323,10 +323,10 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// paged_keep(k_pages, v_pages, tables, lens, paths [batch, depth], out or None) -> lens
+// paged_keep(k_pages, v_pages, tables, lens, paths [batch, depth], held or None, out or None) -> lens
 PyObject *paged_keep(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect_args(n, 6, "paged_keep");
+    expect_args(n, 7, "paged_keep");
     const Pages pages(args[0], args[1], -1, true, true);
     const int dev = pages.k.get_device();
     const Tensor &lens = paged_arg(args[3], "lens", dev);
@@ -334,18 +334,19 @@ PyObject *paged_keep(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int64_t batch = lens.size(0);
     ints_arg(args[3], "lens", dev, at::kInt, batch);
     const Tensor &tables = rows_arg(args[2], "tables", dev, batch), &paths = rows_arg(args[4], "paths", dev, batch);
+    const Tensor *held = args[5] == Py_None ? nullptr : &ints_arg(args[5], "held", dev, at::kInt, batch);
     Tensor out;
-    if (args[5] != Py_None) {
-        out = ints_arg(args[5], "out", dev, at::kInt, batch);
-        for (const Tensor *t : std::initializer_list<const Tensor *>{&lens, &tables, &paths}) TORCH_CHECK(!overlap(out, *t), "gpuk: paged_keep: out overlaps what is read");
+    if (args[6] != Py_None) {
+        out = ints_arg(args[6], "out", dev, at::kInt, batch);
+        for (const Tensor *t : {&lens, &tables, &paths, held}) TORCH_CHECK(!t || !overlap(out, *t), "gpuk: paged_keep: out overlaps what is read");
     }
     {
         NoGil unlocked;
         c10::cuda::CUDAGuard guard(pages.k.device());
         if (!out.defined()) out = empty_like_on(lens, {batch}, at::kInt);
-        check(gpuk_paged_keep(&pages.c, int_size(pages.layers), pages.layer_stride, tables.data_ptr<int>(), batch > 1 ? tables.stride(0) : tables.size(1), int_size(tables.size(1)),
-                              lens.data_ptr<int>(), paths.data_ptr<int>(), batch > 1 ? paths.stride(0) : paths.size(1), int_size(paths.size(1)), out.data_ptr<int>(), int_size(batch),
-                              stream_of(lens)), "paged_keep");
+        check(gpuk_paged_keep_held(&pages.c, int_size(pages.layers), pages.layer_stride, tables.data_ptr<int>(), batch > 1 ? tables.stride(0) : tables.size(1), int_size(tables.size(1)),
+                                   lens.data_ptr<int>(), paths.data_ptr<int>(), batch > 1 ? paths.stride(0) : paths.size(1), int_size(paths.size(1)),
+                                   held ? held->data_ptr<int>() : nullptr, out.data_ptr<int>(), int_size(batch), stream_of(lens)), "paged_keep");
     }
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS

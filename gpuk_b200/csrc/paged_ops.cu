@@ -256,7 +256,7 @@ constexpr int kAhead = 8;      // rows read before the first of them is written
 
 struct KeepParams {
     uint4 *k, *v;
-    const int32_t *tables, *lens, *paths;
+    const int32_t *tables, *lens, *paths, *held;      // held: nullptr, or the pages that the requests have
     int32_t *lens_out;
     int64_t table_stride, path_stride, layer_stride, page_stride, head_stride, row_stride, num_pages;      // strides of the cache in 16-byte vectors
     int width, page_shift, depth, kv_heads, row_vecs;
@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const __grid_constan
     uint4 *cache = (blockIdx.y & 1 ? p.v : p.k) + layer * p.layer_stride;
     const int32_t *path = p.paths + request * p.path_stride, *table = p.tables + request * p.table_stride;
     const int64_t lens = max(p.lens[request], 0), room = static_cast<int64_t>(p.width) << p.page_shift;
+    const int64_t bound = p.held ? static_cast<int64_t>(max(p.held[request], 0)) << p.page_shift : INT64_MAX;
     const bool mine = vec < p.kv_heads * p.row_vecs;
     const int64_t inside = mine ? vec / p.row_vecs * p.head_stride + vec % p.row_vecs : 0;
     // nullptr where there is no such row
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const __grid_constan
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             to[j] = nullptr;
-            ends = ends || node[j] <= last;      // the path's end, or no path
+            ends = ends || node[j] <= last || lens + node[j] >= bound;      // the path's end, or no path, or a node without a page
             if (ends) continue;
             last = node[j];
             if (node[j] != count) {
@@ -364,6 +365,11 @@ extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int
 
 extern "C" int gpuk_paged_keep(const gpuk_pages *pages, int layers, int64_t layer_stride, const int32_t *tables, int64_t table_stride, int table_width, const int32_t *lens,
                                const int32_t *paths, int64_t path_stride, int depth, int32_t *lens_out, int batch, void *stream) {
+    return gpuk_paged_keep_held(pages, layers, layer_stride, tables, table_stride, table_width, lens, paths, path_stride, depth, nullptr, lens_out, batch, stream);
+}
+
+extern "C" int gpuk_paged_keep_held(const gpuk_pages *pages, int layers, int64_t layer_stride, const int32_t *tables, int64_t table_stride, int table_width, const int32_t *lens,
+                                    const int32_t *paths, int64_t path_stride, int depth, const int32_t *held, int32_t *lens_out, int batch, void *stream) {
     if (!pages) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: no pages");
     if (batch < 0 || layers <= 0 || depth < 0 || table_width < 0 || pages->kv_heads <= 0 || pages->head_dim <= 0 || pages->num_pages < 0)
         return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: bad sizes");
@@ -377,7 +383,7 @@ extern "C" int gpuk_paged_keep(const gpuk_pages *pages, int layers, int64_t laye
     if ((reinterpret_cast<uintptr_t>(pages->k) | reinterpret_cast<uintptr_t>(pages->v)) & 15u) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: pointers must be 16-byte aligned");
     for (int64_t s : {layer_stride, pages->page_stride, pages->head_stride, pages->row_stride})
         if (s < 0 || s % 8) return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_keep: strides must be multiples of 8 values");
-    KeepParams p = {static_cast<uint4 *>(pages->k), static_cast<uint4 *>(pages->v), tables, lens, paths, lens_out, table_stride, path_stride, layer_stride / 8,
+    KeepParams p = {static_cast<uint4 *>(pages->k), static_cast<uint4 *>(pages->v), tables, lens, paths, held, lens_out, table_stride, path_stride, layer_stride / 8,
                     pages->page_stride / 8, pages->head_stride / 8, pages->row_stride / 8, pages->num_pages, table_width, page_shift_of(pages->page_size), depth, pages->kv_heads,
                     pages->head_dim / 8};
     // the launch below takes three dimensions

@@ -137,15 +137,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                    0.0 if scale is None else scale, out)
 
 
-def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, paths: torch.Tensor, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, paths: torch.Tensor, *, held: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Makes the accepted path of each request's tree its next cached tokens: new token ``paths[i, j]`` moves to ``lens[i] + j``, in ``k_pages`` and ``v_pages`` of one layer or
     [layers, pages, kv_heads, page_size, head_dim] of all.  A path ascends and ends at its first entry that does not (-1); it names
-    tokens of the last plan only, for only they have pages.  Returns the new lengths."""
-    return _native.paged_keep(k_pages, v_pages, tables, lens, paths, out)
+    tokens of the last plan only, for only they have pages.  ``held`` (``PagedPlan.held``) ends a path at the first token for which no page was to be had: what was never written does
+    not become cached.  Returns the new lengths."""
+    return _native.paged_keep(k_pages, v_pages, tables, lens, paths, held, out)
 
 
 class PagedKVCache:
-    """Pages of all layers, the block tables of ``requests`` requests, and the list of free pages; every tensor stays where it is, so a captured step can be replayed."""
+    """Pages of all layers, the block tables of ``requests`` requests, and the list of free pages; every tensor stays where it is, so a captured step can be replayed.
+
+    Where the pool or a row of the table runs out, tokens of a plan have no slot and NaN logits.  ``append`` and ``keep`` leave them out: a request's cached tokens end in front of the
+    first of them, which can be given again once there are pages."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, requests: int, pages_per_request: int, *, dtype: torch.dtype = torch.bfloat16,
                  device="cuda"):
@@ -162,12 +167,12 @@ class PagedKVCache:
                           free_count_out=self.free_count)
 
     def append(self, new_lens: torch.Tensor) -> None:
-        """All new tokens of the last plan are cached from here on."""
-        self.lens.add_(new_lens)
+        """All new tokens of the last plan that have a page are cached from here on."""
+        torch.clamp(self.lens + new_lens, self.lens, self.held * self.page_size, out=self.lens)      # the upper bound wins
 
     def keep(self, paths: torch.Tensor) -> None:
         """Of the last plan's trees, the paths [requests, depth] are cached from here on (``paged_keep``); what else the pages hold is given back by the next plan."""
-        self.lens.copy_(paged_keep(self.k, self.v, self.tables, self.lens, paths))
+        self.lens.copy_(paged_keep(self.k, self.v, self.tables, self.lens, paths, held=self.held))
 
     def release(self, requests) -> None:
         """Ends requests: their pages go back to the list with the next plan, in which they have no new tokens."""

@@ -467,9 +467,13 @@ int gpuk_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_s
 /*
  * The accepted path of each request's tree: new token path[j] becomes cached token lens + j, in `layers` layers of keys and values.  A path [depth] ascends
  * strictly from 0 or more and ends at the first entry that does not (-1 by habit).  lens_out[i] = lens[i] + its length; lens_out is not lens.
+ * gpuk_paged_keep_held: with held[i] the pages that request i has (gpuk_paged_plan), its path also ends at the first node that they do not reach.  Where pages ran out, a
+ * node behind them was never written, and to count it as cached would hand its place to whatever page comes there later.
  */
 int gpuk_paged_keep(const gpuk_pages *pages, int layers, int64_t layer_stride, const int32_t *tables, int64_t table_stride, int table_width, const int32_t *lens,
                     const int32_t *paths, int64_t path_stride, int depth, int32_t *lens_out, int batch, void *stream);
+int gpuk_paged_keep_held(const gpuk_pages *pages, int layers, int64_t layer_stride, const int32_t *tables, int64_t table_stride, int table_width, const int32_t *lens,
+                         const int32_t *paths, int64_t path_stride, int depth, const int32_t *held, int32_t *lens_out, int batch, void *stream);
 
 /*
  * No counterpart in the reference.  Same job as gpuk_emulated_allreduce_rms (fused op only)

@@ -32,3 +32,130 @@ def test_tiles_behind_the_table_s_end(heads, kv, hd, page, width, ctx, new, dtyp
     b.check(got)
     if not masked:
         b.check(b.run(max_new=1))
+
+
+# ---- pools that run out ------------------------------------------------------------------------------------
+def _state(cache):
+    """The pages of every request and of the list, each once."""
+    held = [[int(x) for x in row[:n]] for row, n in zip(cache.tables.tolist(), cache.held.tolist())]
+    free = cache.free[:int(cache.free_count[0])].tolist()
+    return held, free
+
+
+def _write(cache, plan, g, heads=2):
+    """Random keys and values of the new tokens into their slots; returns them."""
+    n, kv, hd = plan.slots.shape[0], cache.k.shape[2], cache.k.shape[4]
+    x = torch.randn(3, n, max(heads, kv), hd, generator=g).to(cache.k.dtype).cuda()
+    zero = torch.zeros(n, dtype=torch.int64, device="cuda")      # no rotation
+    q = gpuk.rope_paged(x[0, :, :heads].contiguous(), x[1, :, :kv], x[2, :, :kv], zero, plan.slots, gpuk.rope_frequencies(hd, device="cuda"), cache.k[0], cache.v[0])
+    return x[0, :, :heads], q, x[1, :, :kv], x[2, :, :kv]
+
+
+def _attended(q, keys, values):
+    """One token over the keys given, in 64 bits."""
+    s = torch.einsum("hd,nhd->hn", q.double(), keys.double()) / q.shape[-1] ** 0.5
+    return torch.einsum("hn,nhd->hd", torch.softmax(s, -1), values.double())
+
+
+@pytest.mark.parametrize("step", ["append", "keep"])
+def test_tokens_without_a_page_do_not_become_cached(step):
+    """The pool runs out in the middle of a request's new tokens.  What has no page is not counted as cached, so that a page that comes free later, with keys of its last owner, is not taken for
+    it; the next token goes where the cached ones end and sees them and itself."""
+    g = torch.Generator().manual_seed(3)
+    cache = gpuk.PagedKVCache(1, 4, 8, 2, 64, 2, 6)
+    first = _ints([10, 7])
+    plan = cache.plan(first, 17)
+    _, _, k0, v0 = _write(cache, plan, g)
+    cache.append(first)
+    assert cache.lens.tolist() == [10, 7] and cache.held.tolist() == [2, 1]
+    # 14 more tokens of the first request: 6 and 8 of them have pages; a chain, so that both steps keep them all
+    more = _ints([20, 0])
+    plan = cache.plan(more, 20, parents=_ints(list(range(-1, 19))), max_new=20)
+    assert plan.free_count.tolist() == [0, 1] and plan.slots[14:].tolist() == [-1] * 6
+    _, q, k1, v1 = _write(cache, plan, g)
+    assert bool(q[14:].isnan().all())
+    if step == "append":
+        cache.append(more)
+    else:
+        cache.keep(_ints([list(range(20)), [-1] * 20]))
+    assert cache.lens.tolist() == [24, 7]
+    # the second request ends and its page, full of its keys, goes to the first
+    cache.release([1])
+    one = _ints([1, 0])
+    plan = cache.plan(one, 1)
+    assert plan.free_count.tolist() == [0, 0] and plan.positions.tolist() == [24] and cache.held.tolist() == [4, 0]
+    raw, q, k2, v2 = _write(cache, plan, g)
+    got = gpuk.paged_attention(q, cache.k[0], cache.v[0], cache.tables, cache.lens, plan.starts)
+    want = _attended(q[0], torch.cat([k0[:10], k1[:14], k2]), torch.cat([v0[:10], v1[:14], v2]))
+    # weights and the result rounded to bf16 once each, sums of magnitudes of a few units
+    assert float((got[0].double() - want).abs().amax()) <= 2.0 ** -7 * 4
+    cache.append(one)
+    assert cache.lens.tolist() == [25, 0]
+    _status_ok()
+
+
+def test_a_path_ends_at_its_first_token_without_a_page():
+    """Accepted nodes in front of it are kept, those behind it are not, even where the rows that they would move to have pages; a request with all of its pages keeps its path."""
+    g = torch.Generator().manual_seed(4)
+    cache = gpuk.PagedKVCache(1, 5, 8, 2, 64, 2, 6)
+    plan = cache.plan(_ints([4, 9]), 13)
+    _write(cache, plan, g)
+    cache.append(_ints([4, 9]))
+    assert cache.held.tolist() == [1, 2]
+    # trees of 26 and 5 nodes behind 4 and 9 tokens: 30 tokens want four pages, of which three are to be had
+    plan = cache.plan(_ints([26, 5]), 31, parents=_ints([-1] + [0] * 25 + [-1, 0, 0, 1, 3]), max_new=26)
+    assert cache.held.tolist() == [3, 2] and plan.free_count.tolist() == [0, 1] and plan.slots[:26].tolist().index(-1) == 20
+    _, _, k, v = _write(cache, plan, g)
+    cache.keep(_ints([[0, 3, 21, 23], [0, 1, 3, 4]]))
+    assert cache.lens.tolist() == [6, 13]
+    for i, (c, at) in enumerate(((4, [0, 3]), (9, [26, 27, 29, 30]))):
+        for j, node in enumerate(at):
+            page = int(cache.tables[i, (c + j) // 8])
+            assert torch.equal(cache.k[0, page, :, (c + j) % 8], k[node]) and torch.equal(cache.v[0, page, :, (c + j) % 8], v[node])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_pool_that_is_always_short(seed):
+    """Random steps of requests that want more than there is: lengths never pass the pages that are held, no page is lost or twice, and every cached row holds what was written for it."""
+    rng, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    cache = gpuk.PagedKVCache(1, 12, 8, 1, 64, 4, 5)
+    texts = [[] for _ in range(4)]      # the values of the cached tokens
+    for _ in range(25):
+        new = [rng.choice([0, 1, 1, 5, 12]) for _ in range(4)]
+        for i in range(4):
+            if rng.random() < 0.15:
+                cache.release([i])
+                texts[i] = []
+        total = sum(new)
+        tree = rng.random() < 0.5
+        plan = cache.plan(_ints(new), total, parents=_ints([p for n in new for p in range(-1, n - 1)]) if tree else None, max_new=12 if tree else 0)
+        slots, starts = plan.slots.tolist(), plan.starts.tolist()
+        if total:
+            _, _, _, v = _write(cache, plan, g)
+        there = [[j for j in range(n) if slots[starts[i] + j] >= 0] for i, n in enumerate(new)]
+        if tree:      # every other node of the chain: any ascending list is a path to the call
+            paths = [list(range(rng.randint(0, 1), n, rng.randint(1, 2))) for n in new]
+            cache.keep(_ints([p + [-1] * (12 - len(p)) for p in paths]))
+            kept = [[j for j in p if j in there[i]] for i, p in enumerate(paths)]
+        else:
+            cache.append(_ints(new))
+            kept = there
+        for i in range(4):
+            texts[i] += [v[starts[i] + j, 0] for j in kept[i]]
+        assert cache.lens.tolist() == [len(t) for t in texts]
+        held, free = _state(cache)
+        assert sorted(sum(held, []) + free) == list(range(12)) and all(len(t) <= 8 * len(h) for t, h in zip(texts, held))
+        for t, h in zip(texts, held):
+            for j, row in enumerate(t):
+                assert torch.equal(cache.v[0, h[j // 8], 0, j % 8], row)
+
+
+def test_lengths_that_are_held_stay_as_they_are():
+    """Fewer tokens appended than were planned, none, and none with negative counts, which a plan takes for none; a request that fills its pages to the end."""
+    cache = gpuk.PagedKVCache(1, 9, 8, 1, 64, 3, 4)
+    cache.plan(_ints([16, 3, -5]), 19)
+    cache.append(_ints([16, 2, -5]))
+    assert cache.lens.tolist() == [16, 2, 0]
+    cache.plan(_ints([16, 5, 0]), 21)
+    cache.append(_ints([16, 5, 0]))
+    assert cache.lens.tolist() == [32, 7, 0] and cache.held.tolist() == [4, 1, 0]
