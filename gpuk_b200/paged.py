@@ -83,8 +83,9 @@ def scaled_frequencies(rotary: int, theta: float = 10000.0, scaling: Optional[di
     if kind == "bands":
         stay = ((original * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
         return f / factor * (1 - stay) + f * stay, 1.0
+    # the ramp may end beyond the last pair, where all turn more than `low` times: none of them is divided by the whole factor then
     first = max(math.floor(rotary * math.log(original / (high * 2 * math.pi)) / (2 * math.log(theta))), 0)
-    last = min(math.ceil(rotary * math.log(original / (low * 2 * math.pi)) / (2 * math.log(theta))), rotary // 2 - 1)
+    last = min(math.ceil(rotary * math.log(original / (low * 2 * math.pi)) / (2 * math.log(theta))), rotary - 1)
     slow = ((i / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
     return f / factor * slow + f * (1 - slow), 0.1 * math.log(factor) + 1.0
 

@@ -1,0 +1,40 @@
+"""The paged cache at its edges, as far as it needs no GPU: rotary frequencies at the ends of their ramps."""
+import math
+
+import pytest
+
+import gpuk_b200 as gpuk
+
+
+# ---- rotary frequencies --------------------------------------------------------------------------------------
+def _yarn(rotary, theta, factor, low, high, original):
+    """From the definition: a ramp from 0 to 1 along the pairs, between the whole numbers around those that turn `high` and `low` times over the original context, clamped to the values of a
+    head and not to its pairs; 1 is divided by the factor, 0 is left."""
+    pair = lambda turns: rotary * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+    first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), rotary - 1)
+    out = []
+    for i in range(rotary // 2):
+        f, ramp = theta ** (-2 * i / rotary), min(max((i - first) / max(last - first, 0.001), 0.0), 1.0)
+        out.append(f * (1 - ramp) + f / factor * ramp)
+    return out
+
+
+@pytest.mark.parametrize("rotary,theta,original,low,high", [(16, 10000.0, 32768, 1.0, 32.0), (16, 10000.0, 1 << 20, 1.0, 32.0), (32, 10000.0, 131072, 0.5, 64.0), (128, 500000.0, 4096, 1.0, 32.0),
+                                                           (128, 100.0, 8192, 1.0, 32.0), (64, 10000.0, 100, 1.0, 32.0)])
+def test_yarn_beyond_the_last_pair(rotary, theta, original, low, high):
+    """The ramp ends where a pair would turn `low` times, be it beyond the last: pairs that turn more often are never divided by the whole factor."""
+    f, amplitude = gpuk.paged.scaled_frequencies(rotary, theta, {"kind": "yarn", "factor": 16.0, "low": low, "high": high, "original": original})
+    want = _yarn(rotary, theta, 16.0, low, high, original)
+    # a few roundings of 64-bit numbers
+    assert all(abs(a - b) <= 2.0 ** -50 * b for a, b in zip(f.tolist(), want))
+    for i, x in enumerate(f.tolist()):
+        plain = theta ** (-2 * i / rotary)
+        if original * plain / (2 * math.pi) > low:
+            assert x > plain / 16.0 * (1 + 2.0 ** -40)
+    assert amplitude == 0.1 * math.log(16.0) + 1
+
+
+def test_the_last_pair_of_a_short_head():
+    """rotary 16, theta 10000, trained over 32768: the last pair turns 1.65 times, between the ramp's ends 4 and 8, and keeps 1/4 of its own and 3/4 of a sixteenth of its frequency."""
+    f, _ = gpuk.paged.scaled_frequencies(16, 10000.0, {"kind": "yarn", "factor": 16.0, "low": 1.0, "high": 32.0, "original": 32768})
+    assert math.isclose(float(f[7]), 10000.0 ** (-14 / 16) * (0.25 + 0.75 / 16), rel_tol=1e-14)
