@@ -61,7 +61,7 @@ def scaled_frequencies(rotary: int, theta: float = 10000.0, scaling: Optional[di
     ``scaling`` is None or a dict with a ``kind`` and a ``factor``: ``"linear"`` divides all frequencies by the factor; ``"base"`` grows theta so that the slowest pair slows down
     by the factor; ``"bands"`` divides those of pairs that turn fewer than ``low`` times over the ``original`` context, leaves those that turn more than ``high`` times, and
     goes over linearly in between; ``"yarn"`` does the same along the index of the pair (Peng et al., YaRN: efficient context window extension of large language
-    models, 2023) and raises the amplitude to 0.1 ln(factor) + 1."""
+    models, 2023) and raises the amplitude to 0.1 ln(factor) + 1, for factors above 1."""
     i = torch.arange(0, rotary, 2, dtype=torch.float64)
     f = theta ** (-i / rotary)
     if scaling is None:
@@ -87,7 +87,7 @@ def scaled_frequencies(rotary: int, theta: float = 10000.0, scaling: Optional[di
     first = max(math.floor(rotary * math.log(original / (high * 2 * math.pi)) / (2 * math.log(theta))), 0)
     last = min(math.ceil(rotary * math.log(original / (low * 2 * math.pi)) / (2 * math.log(theta))), rotary - 1)
     slow = ((i / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
-    return f / factor * slow + f * (1 - slow), 0.1 * math.log(factor) + 1.0
+    return f / factor * slow + f * (1 - slow), 0.1 * math.log(max(factor, 1.0)) + 1.0
 
 
 def rope_frequencies(rotary: int, theta: float = 10000.0, *, scaling: Optional[dict] = None, device=None) -> RopeFrequencies:

@@ -38,3 +38,9 @@ def test_the_last_pair_of_a_short_head():
     """rotary 16, theta 10000, trained over 32768: the last pair turns 1.65 times, between the ramp's ends 4 and 8, and keeps 1/4 of its own and 3/4 of a sixteenth of its frequency."""
     f, _ = gpuk.paged.scaled_frequencies(16, 10000.0, {"kind": "yarn", "factor": 16.0, "low": 1.0, "high": 32.0, "original": 32768})
     assert math.isclose(float(f[7]), 10000.0 ** (-14 / 16) * (0.25 + 0.75 / 16), rel_tol=1e-14)
+
+
+@pytest.mark.parametrize("factor", [0.5, 1.0])
+def test_a_context_that_does_not_grow_keeps_its_amplitude(factor):
+    _, amplitude = gpuk.paged.scaled_frequencies(64, 10000.0, {"kind": "yarn", "factor": factor, "low": 1.0, "high": 32.0, "original": 4096})
+    assert amplitude == 1.0
