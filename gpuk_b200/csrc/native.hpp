@@ -58,13 +58,15 @@ inline bool plain(PyObject *o, int device) {
     const Tensor &t = THPVariable_Unpack(o);
     return t.is_cuda() && (device < 0 || t.get_device() == device) && t.layout() == at::kStrided && t.is_contiguous();
 }
-// No mode that wants to see operators: tracing, functional transforms, dispatch or function modes.
-inline bool no_modes() {
+// Tracing, a functional transform or a dispatch mode, which want to see what is computed.
+inline bool watched() {
     const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
     static const c10::DispatchKeySet front({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Functionalize,
                                             c10::DispatchKey::Tracer, c10::DispatchKey::Python, c10::DispatchKey::PreDispatch});
-    return !tls.included_.has_any(front) && !c10::impl::TorchDispatchModeTLS::any_modes_set() && at::impl::PythonTorchFunctionTLS::stack_len() == 0;
+    return tls.included_.has_any(front) || c10::impl::TorchDispatchModeTLS::any_modes_set();
 }
+// No mode that wants to see operators: those, and function modes.
+inline bool no_modes() { return !watched() && at::impl::PythonTorchFunctionTLS::stack_len() == 0; }
 
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
 constexpr PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)); }

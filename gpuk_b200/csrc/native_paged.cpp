@@ -11,7 +11,11 @@
 namespace gpuk_native {
 namespace {
 
-// A dense CUDA tensor on the given device (-1: any) that no transform, mode or gradient has an interest in.
+// To a trace the call would not be there: its result would be a constant and nothing be written on replay.  Function modes are not asked: most only say on which device new tensors are made.
+void expect_unwatched(const char *what) {
+    TORCH_CHECK(!watched(), "gpuk::", what, " is no operator that a dispatch mode, a trace or a functional transform could see: call it outside of them");
+}
+// A dense CUDA tensor on the given device (-1: any) that no transform or gradient has an interest in.
 const Tensor &paged_arg(PyObject *o, const char *what, int device) {
     const Tensor &t = tensor_arg(o, what);
     TORCH_CHECK(plain_class(o) && t.layout() == at::kStrided, "gpuk: ", what, " must be a plain tensor");
@@ -158,6 +162,7 @@ class Pool {
 PyObject *paged_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect_args(n, 12, "paged_plan");
+    expect_unwatched("paged_plan");
     const Tensor &lens = paged_arg(args[0], "lens", -1);
     const int dev = lens.get_device();
     TORCH_CHECK(lens.dim() == 1, "gpuk: lens must be one-dimensional");
@@ -225,6 +230,7 @@ PyObject *paged_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect_args(n, 6, "rope");
+    expect_unwatched("rope");
     const Tensor &x = heads_arg(args[0], "x", -1);
     const int dev = x.get_device();
     const Tensor &pos = ints_arg(args[1], "positions", dev, at::kLong, x.size(0)), &turns = paged_arg(args[2], "frequencies", dev);
@@ -249,6 +255,7 @@ PyObject *rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *rope_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect_args(n, 11, "rope_paged");
+    expect_unwatched("rope_paged");
     const Tensor &q = heads_arg(args[0], "q", -1);
     const int dev = q.get_device();
     const Tensor &k = heads_arg(args[1], "k", dev), &v = heads_arg(args[2], "v", dev);
@@ -283,6 +290,7 @@ PyObject *rope_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect_args(n, 11, "paged_attention");
+    expect_unwatched("paged_attention");
     const Tensor &q = heads_arg(args[0], "q", -1);
     const int dev = q.get_device();
     const Pages pages(args[1], args[2], dev, false, false);
@@ -327,6 +335,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *paged_keep(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect_args(n, 7, "paged_keep");
+    expect_unwatched("paged_keep");
     const Pages pages(args[0], args[1], -1, true, true);
     const int dev = pages.k.get_device();
     const Tensor &lens = paged_arg(args[3], "lens", dev);

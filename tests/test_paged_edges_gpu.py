@@ -159,3 +159,41 @@ def test_lengths_that_are_held_stay_as_they_are():
     cache.plan(_ints([16, 5, 0]), 21)
     cache.append(_ints([16, 5, 0]))
     assert cache.lens.tolist() == [32, 7, 0] and cache.held.tolist() == [4, 1, 0]
+
+
+# ---- callers that want to see what is computed ------------------------------------------------------------------
+def _calls():
+    """The five entry points on small arguments, each writing nothing that another reads."""
+    b = _Batch([10], [2], 4, 2, 64, 16)
+    ints = [_ints([3]), _ints([1]), _ints([[0, -1]]), _ints([1]), _ints([2, 3, 0, 0]), _ints([2, 0])]
+    at, f = torch.arange(2, device="cuda"), gpuk.rope_frequencies(64, device="cuda")
+    return b, {"paged_plan": lambda: gpuk.paged_plan(*ints, 16, 1), "rope": lambda: gpuk.rope(b.q, at, f),
+               "rope_paged": lambda: gpuk.rope_paged(b.q, b.q[:, :2], b.q[:, 2:], at, at, f, b.k, b.v),
+               "paged_attention": lambda: gpuk.paged_attention(b.q, b.k, b.v, b.tables, b.lens, b.starts),
+               "paged_keep": lambda: gpuk.paged_keep(b.k, b.v, b.tables, b.lens, _ints([[0]]))}
+
+
+@pytest.mark.parametrize("name", ["paged_plan", "rope", "rope_paged", "paged_attention", "paged_keep"])
+def test_modes_and_tracers_are_refused(name):
+    """A dispatch mode, a trace and a transform would not see the call: a trace would hold its result as a constant and never write the pages."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    b, calls = _calls()
+    with pytest.raises(RuntimeError, match="mode"), Watch():
+        calls[name]()
+    with pytest.raises(RuntimeError, match="mode"):
+        torch.jit.trace(lambda x: x + calls[name]()[0].float().sum(), (torch.zeros(1, device="cuda"),), check_trace=False)
+    with pytest.raises(RuntimeError, match="mode"):
+        torch.func.vmap(lambda x: calls[name]()[0] * x)(torch.ones(2, device="cuda"))
+    # what only says where new tensors go sees nothing of a call and keeps none from it
+    with torch.device("cuda"):
+        calls[name]()
+    with torch.inference_mode():
+        calls[name]()
+    with torch.autocast("cuda"):
+        calls[name]()
+    torch.cuda.synchronize()

@@ -1,7 +1,8 @@
-"""The paged cache at its edges, as far as it needs no GPU: rotary frequencies at the ends of their ramps."""
+"""The paged cache at its edges, as far as it needs no GPU: rotary frequencies at the ends of their ramps, and callers that want to see what is computed."""
 import math
 
 import pytest
+import torch
 
 import gpuk_b200 as gpuk
 
@@ -44,3 +45,23 @@ def test_the_last_pair_of_a_short_head():
 def test_a_context_that_does_not_grow_keeps_its_amplitude(factor):
     _, amplitude = gpuk.paged.scaled_frequencies(64, 10000.0, {"kind": "yarn", "factor": factor, "low": 1.0, "high": 32.0, "original": 4096})
     assert amplitude == 1.0
+
+
+# ---- callers that want to see what is computed ------------------------------------------------------------------
+def test_modes_are_refused_first():
+    """Before the arguments are looked at, by each of the calls."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, f = torch.zeros(3, 2, 64), gpuk.rope_frequencies(64)
+    for call in (lambda: gpuk.paged_plan(x, x, x, x, x, x, 16, 3), lambda: gpuk.rope(x, x, f), lambda: gpuk.rope_paged(x, x, x, x, x, f, x, x),
+                 lambda: gpuk.paged_attention(x, x, x, x, x, x), lambda: gpuk.paged_keep(x, x, x, x, x)):
+        with pytest.raises(RuntimeError, match="dispatch mode"), Watch():
+            call()
+        with pytest.raises(RuntimeError, match="dispatch mode"):
+            torch.func.vmap(lambda y: call())(torch.zeros(2, 1))
+        with pytest.raises(RuntimeError, match="CUDA tensor"), torch.device("cpu"):      # a function mode
+            call()
