@@ -197,3 +197,23 @@ def test_modes_and_tracers_are_refused(name):
     with torch.autocast("cuda"):
         calls[name]()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(grad):
+    """A forward-mode tangent would be dropped; without forward mode there is none to drop."""
+    import torch.autograd.forward_ad as fwd
+
+    b, _ = _calls()
+    at, f = torch.arange(2, device="cuda"), gpuk.rope_frequencies(64, device="cuda")
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        dual = fwd.make_dual(b.q, torch.ones_like(b.q))
+        with pytest.raises(RuntimeError, match="tangent"):
+            gpuk.paged_attention(dual, b.k, b.v, b.tables, b.lens, b.starts)
+        with pytest.raises(RuntimeError, match="tangent"):
+            gpuk.rope(dual, at, f)
+        with pytest.raises(RuntimeError, match="tangent"):
+            gpuk.rope_paged(dual, b.q[:, :2], b.q[:, 2:], at, at, f, b.k, b.v)
+        gpuk.paged_attention(b.q, b.k, b.v, b.tables, b.lens, b.starts)      # tangents elsewhere are no matter
+        with fwd._set_fwd_grad_enabled(False):
+            gpuk.paged_attention(dual, b.k, b.v, b.tables, b.lens, b.starts)
