@@ -351,6 +351,9 @@ class TPDecoder:
             self.frequencies = gpuk.rope_frequencies(a.head_dim, a.rope_theta, scaling=a.rope_scaling, device=self.device)
         hd, heads = a.head_dim, [self.h_local, self.kv_local, self.kv_local]
         h = F.embedding(tokens, self.tok_embeddings)
+        if plan.masks is not None:
+            # A token without a slot has NaN queries, and so NaN scores.  In a tree that passes its table's row it may see no key at all, which is zeros: it is marked from the start.
+            h.masked_fill_((plan.slots < 0)[:, None], math.nan)
         normed, scale = self._norm_only(h, self.layers[0]["attention_norm"], keep=False)      # ragged batches have any number of rows
         for li, layer in enumerate(self.layers):
             k_pages, v_pages = cache.k[li], cache.v[li]

@@ -217,3 +217,27 @@ def test_tangents_are_refused(grad):
         gpuk.paged_attention(b.q, b.k, b.v, b.tables, b.lens, b.starts)      # tangents elsewhere are no matter
         with fwd._set_fwd_grad_enabled(False):
             gpuk.paged_attention(dual, b.k, b.v, b.tables, b.lens, b.starts)
+
+
+# ---- tokens without a place ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("fp8", [False, True])
+def test_logits_of_tokens_without_a_slot(fp8):
+    """Trees larger than the table's row, without cached tokens, so that a node behind its end sees no key at all, and trees that found no page: NaN all the same; the others are numbers."""
+    from tests.test_paged_decoder_gpu import _decoder
+
+    own = not torch.distributed.is_initialized()
+    if own:
+        torch.distributed.init_process_group("gloo", store=torch.distributed.HashStore(), rank=0, world_size=1)
+    try:
+        model = _decoder(gpuk.GPUKDistEnv(group=None, device_id=0), fp8)
+        for pages, requests, per, new in [(9, 2, 1, [20, 6]), (2, 3, 4, [20, 20, 3])]:
+            cache = model.paged_cache(pages=pages, requests=requests, pages_per_request=per, page_size=16)
+            plan = cache.plan(_ints(new), sum(new), parents=_ints([-1] * sum(new)), max_new=20)
+            without = plan.slots < 0
+            assert bool(without.any()) and not bool(without.all())
+            logits = model.forward_paged(torch.arange(sum(new), device="cuda"), cache, plan)
+            assert torch.equal(logits.isnan().all(-1), without) and torch.equal(logits.isnan().any(-1), without)
+        _status_ok()
+    finally:
+        if own:
+            torch.distributed.destroy_process_group()
