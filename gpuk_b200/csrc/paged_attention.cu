@@ -63,7 +63,7 @@ struct Smem {
     uint64_t q_full[2], q_empty, full[kSlotsOf<HD>], empty[kSlotsOf<HD>], s_full[2], p_full[2], o_done[2], together, drained;
     Segment queue[kQueue];
     Start start;
-    uint32_t tmem;
+    uint32_t tmem, gave_up;                      // gave_up: some wait has
     uint32_t poison[3][kMaskedBlocks * 2];       // keys of the masked blocks with a value that is no finite number, of a segment, the next and the one before
 };
 
@@ -82,22 +82,30 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// Barriers by their address in shared memory: the single threads that copy and multiply are bound by the instructions between two waits.
-// A wait gives up after some two seconds.
-__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity) {
+// Barriers by their address in shared memory: the warps that copy and multiply are bound by the instructions between two waits.
+// A wait gives up after some two seconds, each lane by its own clock, or soon where another has: `gave_up` is in shared memory.  What follows a wait (shuffles, loads of tensor memory) is for
+// whole warps, and a lane that left its warp's way would leave the others in it for good.  So a row's lane goes on as if its wait were over, and so do all others behind it, to the end of
+// the segment; the copying lanes go on without copying; and from one segment to the next warps go by a vote.  What comes out then means nothing, which the status says.
+// (A vote behind each wait, in the multiplying warp's way, takes 1 us of 50 for trees of drafts, 2 of 190 for prompts.)
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, uint32_t gave_up) {
     uint64_t began = 0;
     for (uint32_t spin = 1;; ++spin) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
-        if (spin % 1024 == 0) {
+        if (spin % 128 == 0) {
             uint64_t now;
+            asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ok) : "r"(gave_up) : "memory");
+            if (ok) return false;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
             if (began == 0) began = now;
-            else if (now - began > 2000000000ull) return false;
+            else if (now - began > 2000000000ull) break;
         }
     }
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(1) : "memory");
+    return false;
 }
+__device__ __forceinline__ bool vote(bool ok) { return __all_sync(0xffffffffu, ok) != 0; }
 __device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
 __device__ __forceinline__ void commit_at(uint32_t bar) {
@@ -145,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         for (int b = 0; b < 2; ++b) mbar_init(&sm.q_full[b], 1), mbar_init(&sm.s_full[b], 1), mbar_init(&sm.p_full[b], kRows / 32), mbar_init(&sm.o_done[b], 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
         mbar_init(&sm.q_empty, 1), mbar_init(&sm.together, kRows / 32), mbar_init(&sm.drained, 1);
+        sm.gave_up = 0;
         mbar_init_fence();
     }
     if (tid >= kRows + 32)
@@ -159,10 +168,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // behind the allocation: no CTA that follows takes columns one of this grid waits for
     const uint32_t tm = sm.tmem;
-    bool ok = (smem_addr(dyn) & 1023u) == 0;
+    const bool aligned = (smem_addr(dyn) & 1023u) == 0;
+    bool ok = aligned;
 
     const uint32_t full = smem_addr(sm.full), empty = smem_addr(sm.empty), q_full = smem_addr(sm.q_full), s_full = smem_addr(sm.s_full), p_full = smem_addr(sm.p_full),
-                   o_done = smem_addr(sm.o_done), q_empty = smem_addr(&sm.q_empty);
+                   o_done = smem_addr(sm.o_done), q_empty = smem_addr(&sm.q_empty), gave_up = smem_addr(&sm.gave_up);
+    auto wait = [&](uint32_t bar, uint32_t parity) { return wait_at(bar, parity, gave_up); };
+    auto all_well = [&]() { return *static_cast<volatile uint32_t *>(&sm.gave_up) == 0; };
 
     if (warp == kRows / 32 + 1) {      // copies: of a segment K of the first block, Q, and K of the next block before V of each
         const int lane = tid & 31;
@@ -192,18 +204,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             const int inside_mask = rows == kKeys ? (1 << p.page_shift) - 1 : 0;
             auto load = [&](const CUtensorMap *map, int j, int page) {
                 const uint32_t bar = full + 8 * slot;
-                if (!wait_at(empty + 8 * slot, phase)) return false;
-                if (lane == 0) expect_at(bar, kBlockBytes);
+                ok &= wait(empty + 8 * slot, phase);
+                if (lane == 0 && ok) expect_at(bar, kBlockBytes);
                 __syncwarp();
-                if (lane < boxes) {
+                if (lane < boxes && ok) {
                     const int inside = (u.first + j) * kKeys & inside_mask;
                     const uint32_t to = smem_addr(sm.ring) + slot * kBlockBytes + (lane << box_shift) * 128;
 #pragma unroll
                     for (int h = 0; h < kSpans; ++h) tma_load_4d(to + h * kSpanBytes, map, h * 64, inside, u.kvh, page, &sm.full[slot], policy);
                 }
-                ++filled;
+                filled += ok;
                 if (++slot == kSlots) slot = 0, phase ^= 1u;
-                return true;
             };
             // the pages of the next block
             auto next_page = [&](int j) {
@@ -225,40 +236,44 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             };
             if (segments == 0) load_q();      // the first keys wait for the table, those of later segments for nothing
             int page_k = next_page(0);
-            ok = load(&kmap, 0, page_k);
-            if (ok && segments > 0) {
-                ok = wait_at(q_empty, (segments - 1) & 1);
-                if (ok) load_q();
+            load(&kmap, 0, page_k);
+            if (segments > 0) {
+                ok &= wait(q_empty, (segments - 1) & 1);
+                ok = vote(ok && all_well());
+                if (!ok) break;
+                load_q();
             }
-            if (!ok && segments > 0) break;
             ++segments;
-            for (int j = 0; ok && j < u.blocks; ++j) {
+            for (int j = 0; j < u.blocks; ++j) {
                 const int page_v = page_k;
                 if (j + 1 < u.blocks) {
                     page_k = next_page(j + 1);
-                    ok = load(&kmap, j + 1, page_k);
+                    load(&kmap, j + 1, page_k);
                 }
-                if (ok) ok = load(&vmap, j, page_v);
+                load(&vmap, j, page_v);
             }
+            ok = vote(ok);
         }
         if (lane == 0 && p.may_split) p.joints[blockIdx.x] = joint;
         // the end, behind the last segment's scores; and nobody leaves with copies in flight or releases to come
-        if (ok && segments > 0) ok = wait_at(q_empty, (segments - 1) & 1);
+        if (ok && segments > 0) ok = wait(q_empty, (segments - 1) & 1);
         if (ok && lane == 0) {
             sm.queue[segments % kQueue].blocks = 0;
             arrive_at(q_full + 8 * (segments & 1));
         }
-        if (!ok && segments > 0) wait_at(q_full + 8 * ((segments - 1) & 1), ((segments - 1) >> 1) & 1);
-        for (int i = max(0, filled - kSlots); i < filled; ++i) ok = wait_at((ok ? empty : full) + 8 * (i % kSlots), (i / kSlots) & 1) && ok;
+        if (!ok && segments > 0) mbar_wait(&sm.q_full[(segments - 1) & 1], ((segments - 1) >> 1) & 1);
+        for (int i = max(0, filled - kSlots); i < filled; ++i) {
+            if (ok) ok = wait(empty + 8 * (i % kSlots), (i / kSlots) & 1);
+            if (!ok && !mbar_wait(&sm.full[i % kSlots], (i / kSlots) & 1)) break;      // not released: landed at least, however long others have waited
+        }
     } else if (warp == kRows / 32) {   // multiplications: K and V of the ring are used in the order in which they were copied
         // The whole warp goes through the loop and one lane issues, so that descriptors stay in uniform registers: a lane on its own took 80 cycles an instruction.
         constexpr uint32_t s_desc = mma_desc(Half<T>::kFormat, Half<T>::kFormat, kRows, kKeys), o_desc = mma_desc(Half<T>::kFormat, Half<T>::kFormat, kRows, HD, true);
         const uint64_t q_at = kmajor_desc<128>(smem_addr(sm.q)), k_at = kmajor_desc<128>(smem_addr(sm.ring)), v_at = mnmajor_desc(smem_addr(sm.ring), kSpanBytes);
         const uint32_t out_at = __shfl_sync(0xffffffffu, tm, 0) + kOut, scores_at = out_at - kOut;
-        ok = __all_sync(0xffffffffu, ok);
         int slot = 0;
         uint32_t phase = 0, t = 0;      // of the ring; blocks so far
-        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_at(bar, parity)) != 0; };
+        auto wait_all = [&](uint32_t bar, uint32_t parity) { return vote(wait(bar, parity)); };
         auto taken = [&]() {
             if (++slot == kSlots) slot = 0, phase ^= 1u;
         };
@@ -275,21 +290,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             taken();
         };
         for (uint32_t segment = 0; ok; ++segment) {
-            ok = wait(q_full + 8 * (segment & 1), (segment >> 1) & 1);
+            ok = wait_all(q_full + 8 * (segment & 1), (segment >> 1) & 1);
             if (!ok) break;
             const int blocks = __shfl_sync(0xffffffffu, sm.queue[segment % kQueue].blocks, 0);
             if (blocks == 0) break;
-            ok = wait(full + 8 * slot, phase);
+            ok = wait_all(full + 8 * slot, phase);
             tc_fence_after();
             if (ok) scores(t, blocks == 1);
             for (int j = 0; ok && j < blocks; ++j, ++t) {
                 if (j + 1 < blocks) {
-                    ok = wait(full + 8 * slot, phase);
+                    ok = wait_all(full + 8 * slot, phase);
                     tc_fence_after();
                     if (!ok) break;
                     scores(t + 1, j + 2 == blocks);      // into the buffer of P(t - 1), whose product is in front of it
                 }
-                ok = wait(full + 8 * slot, phase) && wait(p_full + 8 * (t & 1), (t >> 1) & 1);
+                ok = wait_all(full + 8 * slot, phase) && wait_all(p_full + 8 * (t & 1), (t >> 1) & 1);
                 tc_fence_after();
                 if (!ok) break;
                 const uint64_t v = v_at + slot * (kBlockBytes / 16);
@@ -304,18 +319,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                 taken();
             }
         }
-        if (!ok) {      // a wait gave up: the row threads do not wait for what was issued, and the tensor memory is about to be freed
-            if (elect_one()) tc_commit(&sm.drained);
-            mbar_wait(&sm.drained, 0);
-        }
+        // where a wait gave up, here or in a row's warp, nobody has waited for what was issued last, and the tensor memory is about to be freed
+        if (elect_one()) tc_commit(&sm.drained);
+        mbar_wait(&sm.drained, 0);
     } else {                           // a row's thread
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, o_at = tm + lanes + kOut;
         const f32x2 scale2 = f2_splat(p.scale_log2);
         const int row_tok = tid / p.group, row_head = tid - row_tok * p.group;
         int t = 0, fill = 0;
-        for (int segment = 0; ok; ++segment) {
-            ok = wait_at(q_full + 8 * (segment & 1), (segment >> 1) & 1);
-            if (!ok) break;
+        for (int segment = 0; aligned; ++segment) {
+            if (!vote(wait(q_full + 8 * (segment & 1), (segment >> 1) & 1) && all_well())) break;
             const Segment u = sm.queue[segment % kQueue];
             if (u.blocks == 0) break;
             const int tok = u.tok0 + row_tok;
@@ -327,9 +340,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             uint32_t *poison = sm.poison[segment % 3];
             if (tid < kMaskedBlocks * 2) sm.poison[(segment + 1) % 3][tid] = 0;      // read last before the barrier of the segment in front
             float m = kLowest, l = 0.f;
-            for (int j = 0; j < u.blocks && ok; ++j, ++t) {
+            for (int j = 0; j < u.blocks; ++j, ++t) {
                 const int block = u.first + j;
-                ok = wait_at(s_full + 8 * (t & 1), (t >> 1) & 1) && ok;      // idle warps too: nobody arrives twice in a phase
+                wait(s_full + 8 * (t & 1), (t >> 1) & 1);      // idle warps too: nobody arrives twice in a phase
                 __syncwarp();
                 if (busy) {
                     tc_fence_after();
@@ -360,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                     if (j == 0) {
                         m = fmaxf(top, kLowest);
                     } else if (__any_sync(0xffffffffu, grown)) {
-                        ok = wait_at(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1) && ok;
+                        wait(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
                         __syncwarp();
                         tc_fence_after();
                         const float f = grown ? exp2_fast(m - top) : 1.f;
@@ -394,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                 if (block >= first_masked) {
                     // values that are none, or that a row may not see and that are no finite numbers, become zeros
                     const int i = fill + (j + 1 < u.blocks ? 2 * j + 2 : 2 * j + 1);
-                    ok = wait_at(full + 8 * (i % kSlots), (i / kSlots) & 1) && ok;
+                    wait(full + 8 * (i % kSlots), (i / kSlots) & 1);
                     uint4 *v = reinterpret_cast<uint4 *>(sm.ring[i % kSlots]);
                     const int keys = static_cast<int>(min(min(static_cast<int64_t>(u.ctx) + u.n, room_of(p)) - static_cast<int64_t>(block) * kKeys, static_cast<int64_t>(kKeys)));
                     constexpr uint32_t e = Half<T>::kExponent;
@@ -431,12 +444,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                 if ((tid & 31) == 0) arrive_at(p_full + 8 * (t & 1));
             }
             fill += 2 * u.blocks;
-            if (ok) ok = wait_at(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
+            wait(o_done + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
             tc_fence_after();
             // all rows' warps have come here, or one of them has given up: a named barrier would wait for it without end
             __syncwarp();
             if ((tid & 31) == 0) arrive_at(smem_addr(&sm.together));
-            if (ok) ok = wait_at(smem_addr(&sm.together), segment & 1);
+            wait(smem_addr(&sm.together), segment & 1);
             if (busy) {
                 uint32_t any = 0;
 #pragma unroll
@@ -463,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                                 const int bit = b * 32 + __ffs(bits) - 1, block = first_masked + bit / kKeys, key = block * kKeys + bit % kKeys;
                                 if (!(seen_of(p, u, tok, block * kKeys) >> (bit % kKeys) & 1)) continue;
                                 const int64_t page = p.tables[u.request * p.table_stride + (key >> p.page_shift)];
+                                if (page < 0 || page >= p.num_pages) continue;      // read as zeros: only behind a wait that gave up can there have been anything else
                                 const T *v = static_cast<const T *>(p.v) + page * p.page_stride + u.kvh * p.head_stride + (key & ((1 << p.page_shift) - 1)) * p.row_stride + c * 32;
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
@@ -492,11 +506,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             }
         }
         // the product before the last has been counted too before the CTA ends
-        if (ok && t > 1) ok = wait_at(o_done + 8 * (t & 1), ((t - 2) >> 1) & 1);
+        if (t > 1) wait(o_done + 8 * (t & 1), ((t - 2) >> 1) & 1);
     }
-    if (!ok) *p.status = 1;
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && !(aligned && all_well())) *p.status = 1;
     if (warp == kRows / 32) {
         tc_fence_after();
         tmem_free<kColumns>(tm);
