@@ -284,7 +284,7 @@ int gpuk::decode_device(const DecodeDevice **out) {
         if (e == cudaSuccess) e = decode_attention_setup(&d);
         if (e == cudaSuccess) e = prefill_attention_setup();
         if (e == cudaSuccess) e = paged_attention_setup();
-        if (e == cudaSuccess) e = paged_ops_setup();
+        if (e == cudaSuccess) e = paged_ops_setup(&d);
         if (e != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "cannot prepare the kernels of a decode step: %s", cudaGetErrorString(e));
         d.status = static_cast<int *>(word);
     }

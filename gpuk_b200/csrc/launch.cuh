@@ -60,6 +60,8 @@ cudaError_t ar_resident_ctas(const ArShape &s, bool emulated, int sm_count, int6
 // Process-wide tuning of the FP8 linear layer (gpuk_set_tuning "fp8_frags_per_warp"): 16-row fragments per warp,
 // 1 or 2; 0 = chosen from the shape.  Defined in fp8_linear.cu.
 extern int fp8_frags_per_warp_tuning;
+// CTAs of a paged plan's cluster at most ("paged_plan_ctas"); 0 = as many as have a place.  Defined in paged_ops.cu.
+extern int paged_plan_ctas_tuning;
 
 // Quantisation policy of an operator quant_type (include/gpuk_b200.h); false for an unknown one.
 bool quant_from_type(int quant_type, Quant *q);

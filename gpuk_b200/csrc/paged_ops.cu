@@ -73,7 +73,7 @@ __device__ V block_before(V v, V *before, V (&warp_sums)[kPlanWarps + 1]) {
 
 // Parents that a CTA keeps at hand beside those of its tokens: of the request that goes on from in front of them.
 constexpr int kBehind = 256;
-constexpr int kPlanCtas = 16;      // of a cluster
+constexpr int kPlanCtas = 16;      // of a cluster, where it has a place
 
 // The mask of a token: `WORDS` words of 32 bits, two of them as one of 64, none without parents.
 template <int WORDS>
@@ -322,16 +322,25 @@ bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 
 }  // namespace
 
-cudaError_t paged_ops_setup() {
+cudaError_t paged_ops_setup(DecodeDevice *d) {
     cudaError_t e = cudaSuccess;
+    d->plan_ctas = kPlanCtas;
     for (int words : {0, 2, kMaxWords}) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_of(words), cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kMaxRequests + 1) * 4);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_of(words), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        while (e == cudaSuccess && d->plan_ctas > 1) {
+            int64_t ctas = 0;
+            if (resident_ctas(plan_of(words), kPlanThreads, d->plan_ctas, d->sms, &ctas, (5 * kMaxRequests + 1) * 4) != cudaSuccess) cudaGetLastError(), ctas = 0;
+            if (ctas >= d->plan_ctas) break;
+            d->plan_ctas /= 2;
+        }
     }
     return e;
 }
 
 }  // namespace gpuk
+
+int gpuk::paged_plan_ctas_tuning = 0;
 
 using namespace gpuk;
 
@@ -356,7 +365,8 @@ extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int
     PlanParams p = {lens, new_lens, held, free_count, parents, tables, free_pages, starts, masks, held_out, free_count_out, positions, slots, table_stride, batch, table_width,
                     page_shift_of(page_size), free_capacity, total, mask_words};
     int ctas = 1;
-    while (ctas < kPlanCtas && total > ctas * kPlanThreads) ctas *= 2;
+    const int most = paged_plan_ctas_tuning && paged_plan_ctas_tuning < d->plan_ctas ? paged_plan_ctas_tuning : d->plan_ctas;
+    while (ctas < most && total > ctas * kPlanThreads) ctas *= 2;
     void *args[] = {&p};
     const cudaError_t e = launch_kernel(plan_of(masks ? mask_words : 0), ctas, kPlanThreads, ctas, false, args, static_cast<cudaStream_t>(stream), (5 * batch + 1) * 4);
     if (e != cudaSuccess) return set_last_error(GPUK_ERR_CUDA, "paged_plan: launch failed: %s", cudaGetErrorString(e));

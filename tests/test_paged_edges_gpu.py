@@ -241,3 +241,23 @@ def test_logits_of_tokens_without_a_slot(fp8):
     finally:
         if own:
             torch.distributed.destroy_process_group()
+
+
+# ---- clusters that have no place ------------------------------------------------------------------------------
+@pytest.mark.parametrize("ctas", [1, 2, 4, 8, 16])
+def test_plans_by_smaller_clusters(ctas):
+    """A part of a GPU may have no place for sixteen CTAs that meet: a plan by any number of them is the same."""
+    from gpuk_b200 import cabi
+    from tests.test_paged_gpu import _check_plan, _random_state
+
+    cabi.check(cabi.lib.gpuk_set_tuning(b"paged_plan_ctas", ctas))
+    try:
+        for batch, page, ctx, new, spare, slack in [(3, 16, 40, 20, 20, 5), (7, 16, 50, 9000, 5000, 3), (1030, 32, 300, 40, 3500, 0)]:
+            _check_plan(*_random_state(random.Random(batch), batch, page, ctx, new, spare, slack))
+        rng = random.Random(ctas)
+        for batch, new in ((300, 64), (90, 256)):
+            state = _random_state(rng, batch, 16, 100, new, batch * new // 10, 2)
+            parents = [rng.choice([-1, j - 1, rng.randint(-1, max(j - 1, -1))]) for n in state[1] for j in range(n)]
+            _check_plan(*state, parents=parents + [-1, -1], max_new=new)
+    finally:
+        cabi.check(cabi.lib.gpuk_set_tuning(b"paged_plan_ctas", 0))

@@ -65,3 +65,11 @@ def test_modes_are_refused_first():
             torch.func.vmap(lambda y: call())(torch.zeros(2, 1))
         with pytest.raises(RuntimeError, match="CUDA tensor"), torch.device("cpu"):      # a function mode
             call()
+
+
+# ---- clusters that have no place ------------------------------------------------------------------------------
+def test_the_cap_on_a_plan_s_cluster():
+    from gpuk_b200 import cabi
+
+    for value, status in ((16, cabi.OK), (1, cabi.OK), (0, cabi.OK), (3, cabi.ERR_INVALID_ARGUMENT), (32, cabi.ERR_INVALID_ARGUMENT), (-1, cabi.ERR_INVALID_ARGUMENT)):
+        assert cabi.lib.gpuk_set_tuning(b"paged_plan_ctas", value) == status
