@@ -155,6 +155,20 @@ class PagedKVCache:
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, requests: int, pages_per_request: int, *, dtype: torch.dtype = torch.bfloat16,
                  device="cuda"):
+        # what the calls of a step would refuse is refused before there is one
+        for name, size, least in (("layers", layers, 0), ("pages", pages, 1), ("kv_heads", kv_heads, 1), ("requests", requests, 0), ("pages_per_request", pages_per_request, 1)):
+            if size < least:
+                raise ValueError(f"gpuk: a paged cache with {name}={size}")
+        if not 8 <= page_size <= 65536 or page_size & (page_size - 1):
+            raise ValueError(f"gpuk: pages of {page_size} tokens; attention is built for powers of two from 8 to 65536")
+        if head_dim not in (64, 128):
+            raise ValueError(f"gpuk: heads of {head_dim}; attention over pages is built for 64 and 128")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"gpuk: a paged cache of {dtype}; it is bfloat16 or float16")
+        if requests > 4096:
+            raise ValueError(f"gpuk: {requests} requests; a plan is built for at most 4096")
+        if pages_per_request * page_size > 0x7fffff00 or requests * pages_per_request > 0x7fffffff:
+            raise ValueError(f"gpuk: tables of {requests} requests with pages_per_request={pages_per_request} are too large")
         self.page_size = page_size
         self.k, self.v = (torch.zeros(layers, pages, kv_heads, page_size, head_dim, dtype=dtype, device=device) for _ in range(2))
         ints = {"dtype": torch.int32, "device": device}

@@ -330,8 +330,10 @@ class TPDecoder:
         return self._reduce_add_norm(partial, h, nxt)
 
     def paged_cache(self, pages: int, requests: int, pages_per_request: int, page_size: int = 64) -> gpuk.PagedKVCache:
-        """An empty cache of this rank's KV heads for ``forward_paged``."""
+        """An empty cache of this rank's KV heads for ``forward_paged``.  Heads of 64 or 128, at most 128 query heads a KV head, bf16 or fp16, pages of a power of two from 8."""
         a = self.args
+        if self.h_local % self.kv_local or self.h_local // self.kv_local > 128:
+            raise ValueError(f"gpuk: {self.h_local} query heads over {self.kv_local} KV heads; attention over pages is built for a whole number up to 128 of each")
         return gpuk.PagedKVCache(a.n_layers, pages, page_size, self.kv_local, a.head_dim, requests, pages_per_request, dtype=a.dtype, device=self.device)
 
     @torch.no_grad()

@@ -73,3 +73,33 @@ def test_the_cap_on_a_plan_s_cluster():
 
     for value, status in ((16, cabi.OK), (1, cabi.OK), (0, cabi.OK), (3, cabi.ERR_INVALID_ARGUMENT), (32, cabi.ERR_INVALID_ARGUMENT), (-1, cabi.ERR_INVALID_ARGUMENT)):
         assert cabi.lib.gpuk_set_tuning(b"paged_plan_ctas", value) == status
+
+
+# ---- caches that attention cannot read ------------------------------------------------------------------------
+@pytest.mark.parametrize("more,text", [({"page_size": 4}, "pages of 4"), ({"page_size": 48}, "pages of 48"), ({"page_size": 1 << 17}, "pages of 131072"), ({"head_dim": 96}, "heads of 96"),
+                                       ({"head_dim": 256}, "heads of 256"), ({"requests": 4097}, "4097 requests"), ({"dtype": torch.float32}, "bfloat16 or float16"), ({"kv_heads": 0}, "kv_heads"),
+                                       ({"pages_per_request": 1 << 27}, "pages_per_request"), ({"layers": -1}, "layers"), ({"pages": 0}, "pages=0"), ({"pages_per_request": 0}, "pages_per_request=0"), ({"requests": -1}, "requests")])
+def test_a_cache_is_refused_when_it_is_made(more, text):
+    """Not by the first attention over it, when a plan has dealt out pages and a layer's keys are written."""
+    good = dict(layers=1, pages=2, page_size=16, kv_heads=2, head_dim=64, requests=3, pages_per_request=2, dtype=torch.float16, device="cpu")
+    gpuk.PagedKVCache(**good)
+    with pytest.raises(ValueError, match=text):
+        gpuk.PagedKVCache(**{**good, **more})
+
+
+@pytest.mark.parametrize("more,text", [({"head_dim": 96}, "heads of 96"), ({"head_dim": 32}, "heads of 32"), ({"dtype": torch.float32}, "bfloat16 or float16"), ({"n_heads": 6, "n_kv_heads": 4}, "6 query heads"),
+                                       ({"n_heads": 129, "n_kv_heads": 1}, "129 query heads")])
+def test_a_decoder_refuses_a_cache_that_it_could_not_read(more, text):
+    from gpuk_b200.tp_model import DecoderArgs, TPDecoder
+
+    class Alone:
+        rank, world_size = 0, 1
+
+    def decoder(**more):
+        return TPDecoder(DecoderArgs(**{**dict(dim=64, n_layers=1, n_heads=2, n_kv_heads=1, head_dim=64, ffn_dim=64, vocab_size=32, max_seq_len=16), **more}), Alone(), device="cpu", fp8=False, max_batch=1)
+
+    assert decoder().paged_cache(4, 2, 2).page_size == 64
+    with pytest.raises(ValueError, match=text):
+        decoder(**more).paged_cache(4, 2, 2)
+    with pytest.raises(ValueError, match="pages of 2"):
+        decoder().paged_cache(4, 2, 2, page_size=2)
