@@ -85,6 +85,7 @@ struct Half<__nv_bfloat16> {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
     }
+    __device__ static float round(float x) { return __uint_as_float(pack(0.f, x)); }      // the upper half, and nothing below
 };
 template <>
 struct Half<__half> {
@@ -96,6 +97,7 @@ struct Half<__half> {
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
     }
+    __device__ static float round(float x) { return __half2float(__float2half_rn(x)); }
 };
 // ---- which parts of which tiles a CTA takes ---------------------------------------------------------
 // Tiles lie one after another, by request, kv head and token, each as long as the keys that it sees and kTileCost more.  A CTA takes an equal share of that line; where a border comes

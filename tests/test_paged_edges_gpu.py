@@ -261,3 +261,24 @@ def test_plans_by_smaller_clusters(ctas):
             _check_plan(*state, parents=parents + [-1, -1], max_new=new)
     finally:
         cabi.check(cabi.lib.gpuk_set_tuning(b"paged_plan_ctas", 0))
+
+
+# ---- rounded weights -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, BF16), (128, F16), (64, F16)])
+def test_a_weight_that_dominates_moves_nothing_by_its_rounding(hd, dtype):
+    """Two keys of different blocks carry each row, the second with a weight of up to 2^7 that the operands' type does not hold, and all values are alike: what comes out is that value, as
+    the sum holds the weight as it was multiplied.  Other keys weigh 2^-32 or less each beside the first; sums of two products and the quotient are off by some 2^-22, which no value's rounding sees."""
+    heads, ctx = 96, 190
+    b = _Batch([ctx], [2], heads, 1, hd, 64, dtype)
+    g = torch.Generator().manual_seed(hd)
+    value = torch.randn(hd, generator=g).to(dtype).cuda()
+    b.v[:] = value
+    b.k[:] = 0
+    b.k[..., 0] = -64.0
+    b.k[int(b.tables[0, 0]), 0, 5] = 0
+    b.k[int(b.tables[0, 2]), 0, 2, 0] = 1.0
+    b.q[:] = 0
+    # log2 of the second weight: 0.5 to 6.9, so the others are at -32 and below, beside the two
+    b.q[..., 0] = (torch.rand(2, heads, generator=g) * 6.4 + 0.5).cuda().to(dtype)
+    got = b.run(scale=0.6931471805599453)
+    assert torch.equal(got, value.expand(2, heads, hd))
