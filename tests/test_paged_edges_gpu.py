@@ -282,3 +282,58 @@ def test_a_weight_that_dominates_moves_nothing_by_its_rounding(hd, dtype):
     b.q[..., 0] = (torch.rand(2, heads, generator=g) * 6.4 + 0.5).cuda().to(dtype)
     got = b.run(scale=0.6931471805599453)
     assert torch.equal(got, value.expand(2, heads, hd))
+
+
+# ---- many requests, and none ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("batch,most", [(1000, 1), (4096, 1), (1500, 3)])
+def test_attention_of_thousands_of_requests(batch, most):
+    """Each lane of the border search looks after a hundred of them; single tokens, and a few each, against a padded batch in 64 bits."""
+    rng, g = random.Random(batch), torch.Generator(device="cuda").manual_seed(batch)
+    page, kv, heads, hd, longest = 16, 2, 4, 64, 40
+    ctx, new = [rng.randint(0, longest - most) for _ in range(batch)], [rng.randint(0, most) if rng.random() < 0.5 else most for _ in range(batch)]
+    ctx[7], width = 700, 48      # one of them is cut into parts
+    total = sum(new)
+    pages = sum(-(-(c + n) // page) for c, n in zip(ctx, new))
+    order, tables, at = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).tolist(), [], 0
+    for c, n in zip(ctx, new):
+        need = -(-(c + n) // page)
+        tables.append(order[at:at + need] + [-1] * (width - need))
+        at += need
+    k, v = (torch.randn(pages, kv, page, hd, generator=g, device="cuda").to(BF16) for _ in range(2))
+    q = torch.randn(total, heads, hd, generator=g, device="cuda").to(BF16)
+    starts = torch.tensor([0] + new).cumsum(0).int().cuda()
+    t, lens = _ints(tables), _ints(ctx)
+    got = gpuk.paged_attention(q, k, v, t, lens, starts)
+    _status_ok()
+    request = torch.repeat_interleave(torch.arange(batch, device="cuda"), torch.tensor(new, device="cuda"))
+    index = torch.arange(total, device="cuda") - starts[request]
+    for part in torch.arange(total, device="cuda").split(512):
+        r = request[part]
+        kk, vv = (c[t[r].long().clamp(min=0)].transpose(2, 3).reshape(len(r), width * page, kv, hd).repeat_interleave(heads // kv, 2).double() for c in (k, v))
+        s = torch.einsum("thd,tnhd->thn", q[part].double(), kk) / hd ** 0.5
+        seen = torch.arange(width * page, device="cuda") <= (lens[r] + index[part])[:, None]
+        p = torch.softmax(s.masked_fill(~seen[:, None], float("-inf")), -1)
+        want, size = torch.einsum("thn,tnhd->thd", p, vv), torch.einsum("thn,tnhd->thd", p, vv.abs())
+        # each weight and the result are rounded once
+        assert bool(((got[part].double() - want).abs() <= size * (2.0 ** -8 + 2.0 ** -15) + want.abs() * 2.0 ** -8 + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_step_of_nothing(fp8):
+    """A server whose requests have all ended: no rows, no logits, and nothing changes."""
+    from tests.test_paged_decoder_gpu import _decoder
+
+    own = not torch.distributed.is_initialized()
+    if own:
+        torch.distributed.init_process_group("gloo", store=torch.distributed.HashStore(), rank=0, world_size=1)
+    try:
+        model = _decoder(gpuk.GPUKDistEnv(group=None, device_id=0), fp8)
+        cache = model.paged_cache(pages=4, requests=2, pages_per_request=2, page_size=16)
+        none = _ints([0, 0])
+        logits = model.forward_paged(torch.zeros(0, dtype=torch.int64, device="cuda"), cache, cache.plan(none, 0))
+        cache.append(none)
+        assert logits.shape == (0, 512) and cache.lens.tolist() == [0, 0] and cache.free_count.tolist() == [4, 0]
+        _status_ok()
+    finally:
+        if own:
+            torch.distributed.destroy_process_group()
