@@ -351,6 +351,7 @@ extern "C" int gpuk_paged_plan(const int32_t *lens, const int32_t *new_lens, int
         return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_plan: bad sizes");
     if (!power_of_two(page_size) || page_size > 65536) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_plan: pages of %d tokens; built for powers of two up to 65536", page_size);
     if (batch > kMaxRequests) return set_last_error(GPUK_ERR_UNSUPPORTED, "paged_plan: %d requests; built for at most %d", batch, kMaxRequests);
+    if (total == 0) parents = nullptr, masks = nullptr;      // of no tokens there may be neither, or only an address
     if (!parents != !masks || (masks && (mask_words < 1 || mask_words > kMaxWords)))
         return set_last_error(GPUK_ERR_INVALID_ARGUMENT, "paged_plan: parents come with masks of 1 to %d words", kMaxWords);
     if (static_cast<int64_t>(batch) * table_width > 0x7fffffffll || static_cast<int64_t>(table_width) * page_size > 0x7fffff00ll)

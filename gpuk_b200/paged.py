@@ -156,7 +156,7 @@ class PagedKVCache:
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, requests: int, pages_per_request: int, *, dtype: torch.dtype = torch.bfloat16,
                  device="cuda"):
         # what the calls of a step would refuse is refused before there is one
-        for name, size, least in (("layers", layers, 0), ("pages", pages, 1), ("kv_heads", kv_heads, 1), ("requests", requests, 0), ("pages_per_request", pages_per_request, 1)):
+        for name, size, least in (("layers", layers, 1), ("pages", pages, 1), ("kv_heads", kv_heads, 1), ("requests", requests, 0), ("pages_per_request", pages_per_request, 1)):
             if size < least:
                 raise ValueError(f"gpuk: a paged cache with {name}={size}")
         if not 8 <= page_size <= 65536 or page_size & (page_size - 1):

@@ -337,3 +337,20 @@ def test_a_step_of_nothing(fp8):
     finally:
         if own:
             torch.distributed.destroy_process_group()
+
+
+def test_trees_without_nodes():
+    """A plan for trees of which there are none, and what follows it: pages still come back."""
+    cache = gpuk.PagedKVCache(1, 4, 8, 2, 64, 2, 3)
+    cache.plan(_ints([9, 3]), 12)
+    cache.append(_ints([9, 3]))
+    cache.release([0])
+    plan = cache.plan(_ints([0, 0]), 0, parents=_ints([]), max_new=5)
+    assert plan.masks.shape == (0, 1) and plan.starts.tolist() == [0, 0, 0] and cache.held.tolist() == [0, 1] and cache.free_count.tolist() == [3, 0]
+    q = torch.zeros(0, 4, 64, dtype=BF16, device="cuda")
+    q = gpuk.rope_paged(q, q[:, :2], q[:, :2], plan.positions, plan.slots, gpuk.rope_frequencies(64, device="cuda"), cache.k[0], cache.v[0])
+    assert gpuk.paged_attention(q, cache.k[0], cache.v[0], cache.tables, cache.lens, plan.starts, masks=plan.masks).shape == (0, 4, 64)
+    cache.keep(_ints([[-1], [-1]]))
+    assert cache.lens.tolist() == [0, 3]
+    empty = gpuk.paged_plan(_ints([]), _ints([]), _ints([]).view(0, 4), _ints([]), _ints([3, 2]), _ints([2, 0]), 16, 2, parents=_ints([7, -1]), max_new=40)
+    assert empty.slots.tolist() == [-1, -1] and not bool(empty.masks.any()) and empty.masks.shape == (2, 2)

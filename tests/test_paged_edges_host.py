@@ -78,7 +78,7 @@ def test_the_cap_on_a_plan_s_cluster():
 # ---- caches that attention cannot read ------------------------------------------------------------------------
 @pytest.mark.parametrize("more,text", [({"page_size": 4}, "pages of 4"), ({"page_size": 48}, "pages of 48"), ({"page_size": 1 << 17}, "pages of 131072"), ({"head_dim": 96}, "heads of 96"),
                                        ({"head_dim": 256}, "heads of 256"), ({"requests": 4097}, "4097 requests"), ({"dtype": torch.float32}, "bfloat16 or float16"), ({"kv_heads": 0}, "kv_heads"),
-                                       ({"pages_per_request": 1 << 27}, "pages_per_request"), ({"layers": -1}, "layers"), ({"pages": 0}, "pages=0"), ({"pages_per_request": 0}, "pages_per_request=0"), ({"requests": -1}, "requests")])
+                                       ({"pages_per_request": 1 << 27}, "pages_per_request"), ({"layers": 0}, "layers=0"), ({"pages": 0}, "pages=0"), ({"pages_per_request": 0}, "pages_per_request=0"), ({"requests": -1}, "requests")])
 def test_a_cache_is_refused_when_it_is_made(more, text):
     """Not by the first attention over it, when a plan has dealt out pages and a layer's keys are written."""
     good = dict(layers=1, pages=2, page_size=16, kv_heads=2, head_dim=64, requests=3, pages_per_request=2, dtype=torch.float16, device="cpu")
@@ -103,3 +103,14 @@ def test_a_decoder_refuses_a_cache_that_it_could_not_read(more, text):
         decoder(**more).paged_cache(4, 2, 2)
     with pytest.raises(ValueError, match="pages of 2"):
         decoder().paged_cache(4, 2, 2, page_size=2)
+
+
+def test_masks_of_no_tokens_need_no_parents():
+    """As far as the call looks at its arguments: with too many requests it goes no further."""
+    from gpuk_b200 import cabi
+    from tests.test_paged_host import P, _plan
+
+    for parents, masks in ((None, P), (P, None), (None, None), (P, P)):
+        assert _plan(total=0, parents=parents, masks=masks, words=1, positions=None, slots=None, free=None) == cabi.ERR_INVALID_ARGUMENT and "null" in cabi.last_error()
+        if not parents != (not masks):
+            assert _plan(total=1, parents=parents, masks=masks, words=1) == cabi.ERR_INVALID_ARGUMENT and "masks" in cabi.last_error()
