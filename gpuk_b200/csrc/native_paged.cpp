@@ -22,8 +22,10 @@ const Tensor &paged_arg(PyObject *o, const char *what, int device) {
     TORCH_CHECK(plain_class(o) && t.layout() == at::kStrided, "gpuk: ", what, " must be a plain tensor");
     TORCH_CHECK(t.is_cuda(), "gpuk: ", what, " must be a CUDA tensor");
     TORCH_CHECK(device < 0 || t.get_device() == device, "gpuk: ", what, " is on another device");
-    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), "gpuk: ", what, " has a forward-mode tangent, which the paged cache's calls would drop");
-    TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()), "gpuk: ", what, " requires a gradient, and the paged cache's calls have none: call them under torch.no_grad()");
+    if (t.unsafeGetTensorImpl()->autograd_meta()) {      // few tensors have any
+        TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()), "gpuk: ", what, " requires a gradient, and the paged cache's calls have none: call them under torch.no_grad()");
+        TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), "gpuk: ", what, " has a forward-mode tangent, which the paged cache's calls would drop");
+    }
     return t;
 }
 const Tensor &ints_arg(PyObject *o, const char *what, int device, at::ScalarType type, int64_t count) {
