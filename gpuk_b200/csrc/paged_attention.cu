@@ -4,8 +4,8 @@
 // itself or those that its bits in `masks` name (in a tree: its ancestors and itself).  softmax(scale * q k^T) v, with a running maximum and sum over blocks of 64 keys.
 //
 // The rows of a tile are pairs of a token and a query head of one kv head's group, tokens outermost: 128 rows are 128 / group tokens, so that a page is read once for a tree of
-// that many nodes, and up to 128 rows cost the tensor pipe less than the page costs HBM (128 operations a byte; the pipe has 250 for each that HBM delivers).  Calls with no
-// more tokens than requests, whose tiles would be nearly empty, go to paged_decode.cu.
+// that many nodes, and up to 128 rows cost the tensor pipe less than the page costs HBM (128 operations a byte; the pipe has 250 for each that HBM delivers).  Calls
+// whose requests have a token each, so that tiles would be nearly empty, go to paged_decode.cu: single_tokens below says which.
 //
 //   * scores go to one of two buffers in tensor memory, so that the next block's are multiplied while a thread per row works on this one's; the probabilities go back into the
 //     same columns, from where they are the first operand of O += P V.  256 columns and 113 KiB a CTA: two CTAs an SM hide each other's waits.
@@ -24,10 +24,11 @@
 // fp32 scores, maxima, sums and outputs.  Probabilities are rounded to the operands' type for the second product; in fp16 they are held times 2^8, so that small
 // ones do not fall under its smallest numbers.
 //
-// Measured (64 / 8 heads of 128, pages of 16 and 64): 2 prompts of 2048 behind 0 and 1000 cached tokens, with 4 single tokens, 186 us, 970 TFLOP/s of what the masks leave, 0.58 of the measured
-// bf16 rate; 8 trees of 33 to 64 nodes over 2000 keys 50; 13 nodes over 31 000 keys of 32 / 8 heads of 64, 29.  What bounds it: for prompts the tensor pipe, which takes as long for a product with 64 columns
-// as for one with 128, so that the scores of 64 keys cost as much as their 128 outputs twice over (half the score products left out of a copy: 138 us; the exponentials left out: 169).  Blocks of 128 keys
-// with two score buffers would need 384 columns a CTA, and so one CTA an SM; with one buffer nothing is multiplied while the rows work on it, and the prompts take 220; one CTA an SM with three
+// Measured (64 / 8 heads of 128, pages of 16 and 64): 2 prompts of 2048 behind 0 and 1000 cached tokens, with 4 single tokens, 224 us a pass among others, where the power limit
+// holds the clock: 800 TFLOP/s of what the masks leave, 0.48 of the measured bf16 rate; 190 in the first milliseconds.  8 trees of 33 to 64 nodes over 2000 keys 58, and 50.5 where three states in turn
+// leave their pages in L2; 13 nodes over 31 000 keys of 32 / 8 heads of 64, 29.  What bounds it: for prompts the tensor pipe, which takes as long for a product with 64 columns
+// as for one with 128, so that the scores of 64 keys cost as much as their 128 outputs twice over (half the score products left out of a copy: 138 us where it took 186; the exponentials left out: 169).  Blocks of 128 keys
+// with two score buffers would need 384 columns a CTA, and so one CTA an SM; with one buffer nothing is multiplied while the rows work on it, and the prompts took 220; one CTA an SM with three
 // buffers, whose row threads take the blocks in turn with a second 128, takes 320 (long prompts 1.2 times as long), since nothing hides a tile's start and end.  For trees and one long context some
 // 9 us of a call are the start of its CTAs, the parts' outputs and the join.  An exponential by polynomial for a quarter of the scores, and two threads a row, did not help: neither unit is the bound.
 #include <cuda_runtime.h>

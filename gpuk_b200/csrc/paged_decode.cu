@@ -1,4 +1,5 @@
-// Attention of single new tokens over pages of a KV cache: what paged_attention.cu computes, for calls with no more tokens than requests and at most 16 query heads per kv head.
+// Attention of single new tokens over pages of a KV cache: what paged_attention.cu computes, for calls without masks and with at most 16 query heads per kv head that say of their requests that
+// each has at most one (max_new 1), or say nothing and have no more tokens than requests.  Right for any number of them, whatever was said.
 //
 // A tile is one token's heads of one kv head's group, at most 16 rows.  It is bound by HBM, and where a call is small by the time from its launch to its last store; the fifth-generation tensor
 // core, whose tiles have 128 rows and whose set-up (tensor memory, barriers, maps) takes microseconds, has nothing to give here.  So, as for the contiguous cache (attention.cu):

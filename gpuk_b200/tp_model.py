@@ -175,7 +175,9 @@ class TPDecoder:
             inv, amplitude = gpuk.paged.scaled_frequencies(hd, a.rope_theta, a.rope_scaling)
         freqs = torch.outer(torch.arange(a.max_seq_len * 2, dtype=inv.dtype), inv)
         self.cos, self.sin = ((f * amplitude).float().to(self.device) for f in (freqs.cos(), freqs.sin()))
-        self.frequencies = None      # the same for positions in a paged cache, once it is used
+        # For positions in a paged cache, once it is used: exact turns at any position.  The table above has fp32 products of position and frequency where nothing is scaled (the reference's), so
+        # the two drift apart with the position: by some 2^-23 of an angle (1e-4 at position 2000).
+        self.frequencies = None
         self._zeros = {}
         # the elementwise steps between the projections as this library's kernels (csrc/decoder_ops.cu)
         self.own_elementwise = fused and self.device.type == "cuda" and a.dtype == torch.bfloat16 and hd % 16 == 0 and a.ffn_dim // w % 8 == 0
